@@ -1,0 +1,848 @@
+"""Losses and records over vocabulary logits, against 64-bit definitions.
+
+Tolerances, for every V up to 131072. A thread adds at most 128 terms to one
+of its sums and some 20 joins follow, each addition off by 2^-24; a term
+2^((x-m)c) is off by 2^-23 from the instruction and by 2^-23 |a| ln 2 from
+its argument a, and the mean of |a| ln 2 under the softmax is at most
+ln V < 12. S, and with it a log-probability, is off by at most
+(128 + 20 + 2 + 2 * 12) 2^-24 < 200 * 2^-24 = LP. A probability as small as
+e^-88 has an argument off by 88 * 2^-23, so q is off by at most LP + 88 * 2^-23
+< 2.3e-5 of itself, and the coefficient of a row (an exponential of an lp) by
+2 LP of itself: a gradient a (q - p) by 6e-5 (|a| q + |gradient|), and by half
+a step of its type. fp16 has steps of 2^-24 below its normal range.
+"""
+import math
+
+import pytest
+import torch
+
+from vantage6_amd.ops.distill import distill_loss, topk_logits
+from vantage6_amd.ops.preference import policy_loss, preference_loss
+
+LP = 200 * 2.0 ** -24
+GRAD = 6e-5
+CPU_GPU = [pytest.param("cpu"), pytest.param("cuda", marks=pytest.mark.gpu)]
+TYPES = [torch.bfloat16, torch.float16, torch.float32]
+# (B, T, V): one token, a vocabulary of one, below a vector, odd, several
+# segments, the models' vocabularies
+SHAPES = [(1, 1, 1), (1, 2, 7), (2, 3, 257), (3, 5, 4099), (2, 2, 30522),
+          (1, 3, 128256), (40, 30, 613)]
+
+
+def need(device):
+    if device == "cuda" and not torch.cuda.is_available():
+        pytest.skip("needs a GPU")
+
+
+def make_logits(B, T, V, dtype, device, seed=0, scale=3.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(B, T, V, generator=g) * scale).to(dtype).to(device)
+
+
+def half_step(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def check_grad(got, want, a, q):
+    """got [.., V] against want (64 bits), a [..] the row's coefficient."""
+    assert got.shape == want.shape
+    least = 2.0 ** -24 if got.dtype == torch.float16 else 1e-37
+    want, a, q = want.double().cpu(), a.double().cpu().abs()[..., None], q.cpu()
+    tol = (half_step(got.dtype) + GRAD) * want.abs() + GRAD * a * q + least
+    err = (got.double().cpu() - want).abs()
+    assert (err <= tol).all(), (err - tol).max().item()
+
+
+def softmax64(logits, t=1.0):
+    x = logits.detach().cpu().double() / t
+    return torch.log_softmax(x, -1)
+
+
+# ------------------------------------------------------------------------ topk
+def topk_oracle(logits, k):
+    """By value, then by place; NaN above all, -0 equal to 0."""
+    x = logits.detach().cpu().double()
+    values, places = [], []
+    for row in x.reshape(-1, x.shape[-1]).tolist():
+        order = sorted(range(len(row)), key=lambda j: (
+            -(math.inf if row[j] != row[j] else row[j]),
+            0 if row[j] != row[j] else 1, j))
+        # a NaN sorts with +inf by value and before it by the flag
+        places.append(order[:k])
+        values.append([row[j] for j in order[:k]])
+    shape = (*x.shape[:-1], k)
+    return torch.tensor(values, dtype=torch.float64).view(shape), torch.tensor(places).view(shape)
+
+
+def check_topk(logits, k, t=1.0):
+    got = topk_logits(logits, k, t)
+    values, places = topk_oracle(logits, k)
+    assert got.values.dtype == logits.dtype and got.indices.dtype == torch.int64
+    assert torch.equal(got.indices.cpu(), places)
+    assert torch.equal(got.values.cpu().double().nan_to_num(7e77), values.nan_to_num(7e77))
+    lse = torch.logsumexp(logits.detach().cpu().double() / t, -1)
+    torch.testing.assert_close(got.logsumexp.cpu().double(), lse, rtol=2.0 ** -23,
+                               atol=LP, equal_nan=True)
+
+
+@pytest.mark.parametrize("device", CPU_GPU)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("R,V,k", [(1, 1, 1), (3, 5, 5), (2, 8, 3), (5, 257, 256),
+                                   (4, 1001, 128), (2, 4099, 1), (3, 30522, 64),
+                                   (1, 128256, 256), (2, 131075, 17)])
+def test_topk(device, dtype, R, V, k):
+    need(device)
+    check_topk(make_logits(1, R, V, dtype, device)[0], k, 1.0 if R % 2 else 2.0)
+
+
+@pytest.mark.parametrize("device", CPU_GPU)
+@pytest.mark.parametrize("dtype", TYPES)
+def test_topk_ties_and_masks(device, dtype):
+    """Constant rows, few finite logits, the type's lowest value, NaN, +-0."""
+    need(device)
+    V = 5003
+    x = make_logits(1, 8, V, dtype, "cpu")[0]
+    x[0] = 1.5  # all equal
+    x[1] = float("-inf")
+    x[1, 77] = -2.0  # one finite
+    x[2] = torch.finfo(dtype).min
+    x[2, 4000] = 0.5
+    x[3, 100] = x[3, 4000] = float("nan")
+    x[3, 50] = float("inf")
+    x[4] = torch.where(torch.arange(V) % 2 == 0, 0.0, -0.0).to(dtype)
+    x[5] = float("-inf")
+    x[6, 1000:] = -3.0  # a long run of equal logits behind a few
+    x[6, :1000] = -5.0
+    x[6, :3] = 4.0
+    x[7, 4992:] = 9.0  # the largest in the last, partial vector
+    check_topk(x.to(device), 12)
+
+
+@pytest.mark.parametrize("device", CPU_GPU)
+def test_topk_layouts(device):
+    need(device)
+    x = make_logits(3, 6, 515, torch.bfloat16, device)
+    for view in (x[:, :-1], x[:, 1:, :512], x[:, :, 1:], x.transpose(0, 1), x[0, 0],
+                 x[:1].expand(3, 6, 515), x[..., ::2], x.view(3, 2, 3, 515)):
+        check_topk(view, 5)
+    empty = topk_logits(x[:, :0], 3)
+    assert empty.values.shape == empty.indices.shape == (3, 0, 3)
+    assert empty.logsumexp.shape == (3, 0)
+
+
+# --------------------------------------------------------------------- distill
+def distill_oracle(logits, values, indices, lse, t, mask):
+    """(loss of each row, live, gradient of the sum, coefficient), 64 bits."""
+    V = logits.shape[-1]
+    x = logits.detach().cpu().double().reshape(-1, V) / t
+    K = indices.shape[-1]
+    v = values.cpu().double().reshape(-1, K) / t
+    idx = indices.cpu().long().reshape(-1, K)
+    m = (torch.ones(len(x), dtype=torch.bool) if mask is None else mask.cpu().reshape(-1))
+    L = None if lse is None else lse.cpu().double().reshape(-1)
+    loss, live = torch.zeros(len(x), dtype=torch.float64), torch.zeros(len(x), dtype=torch.bool)
+    grad = torch.zeros_like(x)
+    for r in range(len(x)):
+        use = (idx[r] >= 0) & (v[r] > -math.inf)
+        if not m[r] or not use.any():
+            continue
+        live[r] = True
+        lq = torch.log_softmax(x[r], -1)
+        lp = v[r][use] - (torch.logsumexp(v[r][use], -1) if L is None else L[r])
+        p, at = lp.exp(), idx[r][use]
+        loss[r] = torch.where(p > 0, p * (lp - lq[at]), 0.0).sum()
+        target = torch.zeros(V, dtype=torch.float64).scatter_add_(0, at, p)
+        # -sum p log q - rest log q_out, with any sum of p: mass q - p - rest q_out
+        q, mass = lq.exp(), p.sum()
+        if L is not None:
+            inside = torch.zeros(V, dtype=torch.bool)
+            inside[idx[r][idx[r] >= 0]] = True
+            rest = (1 - p.sum()).clamp_min(0)
+            if (x[r][~inside] > -math.inf).any():
+                log_out = torch.logsumexp(lq[~inside], -1)
+                loss[r] += torch.xlogy(rest, rest) - rest * log_out
+                # q_j rest / q_out, from logarithms as q_out may be tiny
+                mass = mass + rest
+                q = torch.where(inside, q, q - rest / mass * (lq - log_out).exp())
+        grad[r] = t * (mass * q - target)
+        loss[r] *= t * t
+    rows = logits.shape[:-1]
+    return loss.view(rows), live.view(rows), grad.view(logits.shape)
+
+
+def make_record(logits, k, t, seed=1, tail=True):
+    g = torch.Generator().manual_seed(seed)
+    teacher = logits.detach().cpu().float() + torch.randn(logits.shape, generator=g)
+    values, indices = teacher.topk(k, -1)
+    lse = torch.logsumexp(teacher / t, -1) if tail else None
+    return (values.to(logits.dtype).to(logits.device), indices.to(logits.device),
+            None if lse is None else lse.to(logits.device))
+
+
+def check_distill(logits, values, indices, lse, t=1.0, mask=None, reduction="mean", up=None):
+    x = logits.detach().requires_grad_(True) if logits.is_leaf else logits
+    loss = distill_loss(x, values, indices, lse, temperature=t, mask=mask, reduction=reduction)
+    rows, live, grad = distill_oracle(logits, values, indices, lse, t, mask)
+    assert loss.dtype == torch.float32
+    n = max(int(live.sum()), 1) if reduction == "mean" else 1
+    want = rows if reduction == "none" else rows.sum() / n
+    # KL: sum p (log p - lp), each lp off by LP/t at most: t^2 LP and a rounding
+    lim = 2 * t * t * LP * (1 if reduction != "sum" else max(int(live.sum()), 1))
+    torch.testing.assert_close(loss.detach().cpu().double(), want, rtol=2.0 ** -22, atol=lim)
+    if up is None:
+        up = torch.ones_like(loss)
+    got, = torch.autograd.grad(loss, x, up)
+    scale = up.cpu().double()[..., None] if reduction == "none" else up.cpu().double() / n
+    q = torch.where(live[..., None], softmax64(logits, t).exp(), 0.0)
+    if lse is not None:
+        # outside the record the gradient is q_out-normalised: q + rest * q / q_out
+        q = q + grad.abs() / t
+    coef = torch.ones(logits.shape[:-1], dtype=torch.float64) * t * (
+        up.cpu().double() if reduction == "none" else up.item() / n)
+    check_grad(got, grad * scale, coef, q)
+    if not live.all():
+        assert (got.cpu()[~live] == 0).all()
+    return loss.detach(), got
+
+
+@pytest.mark.parametrize("device", CPU_GPU)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("tail", [False, True])
+def test_distill(device, dtype, shape, tail):
+    need(device)
+    B, T, V = shape
+    t = 2.0 if T % 2 else 1.0
+    x = make_logits(B, T, V, dtype, device)
+    k = min(V, 1 if B == 1 and T == 1 else 19)
+    values, indices, lse = make_record(x, k, t, tail=tail)
+    mask = None
+    if B > 1:
+        mask = (torch.arange(T)[None] < torch.randint(1, T + 1, (B, 1),
+                                                      generator=torch.Generator().manual_seed(5)))
+        mask = mask.to(device)
+    scale = 512.0 if dtype == torch.float16 else 1.0
+    check_distill(x, values, indices, lse, t, mask,
+                  up=torch.tensor(scale, device=device))
+
+
+@pytest.mark.parametrize("device", CPU_GPU)
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+@pytest.mark.parametrize("tail", [False, True])
+def test_distill_reductions_and_upstream(device, reduction, tail):
+    need(device)
+    x = make_logits(2, 4, 1023, torch.float32, device)
+    values, indices, lse = make_record(x, 6, 1.0, tail=tail)
+    up = torch.randn(2, 4, generator=torch.Generator().manual_seed(3)).to(device)
+    check_distill(x, values, indices.int(), lse, 1.0, None, reduction,
+                  up if reduction == "none" else torch.tensor(-3.5, device=device))
+
+
+@pytest.mark.parametrize("device", CPU_GPU)
+@pytest.mark.parametrize("tail", [False, True])
+def test_distill_odd_records(device, tail):
+    """Absent entries, -inf values, the same index twice, an empty record, a
+    masked row of NaN and inf, a record of the whole row, masked logits."""
+    need(device)
+    V, k = 300, 300
+    x = make_logits(1, 8, V, torch.float32, "cpu")[0]
+    teacher = x + 0.5
+    values, indices = teacher.topk(k, -1)
+    lse = torch.logsumexp(teacher, -1) if tail else None
+    values, indices = values[:, :9].clone(), indices[:, :9].clone()
+    indices[0, 3:] = -1  # a short record
+    values[1, 2] = float("-inf")
+    indices[2, 4] = indices[2, 1]  # the same place twice
+    indices[3] = -1  # nothing
+    values[4] = float("-inf")  # nothing either
+    mask = torch.ones(8, dtype=torch.bool)
+    mask[5] = False
+    x[5, ::3] = float("nan")
+    x[5, 1::3] = float("inf")
+    outside = torch.ones(V, dtype=torch.bool)
+    outside[indices[6]] = False
+    x[6, outside] = float("-inf")  # no mass outside the record
+    x[7, outside] = torch.finfo(torch.float32).min
+    args = [None if a is None else a.to(device) for a in (x, values, indices, lse)]
+    check_distill(*args, 1.0, mask.to(device))
+    # no row counts
+    loss, grad = check_distill(*args, 1.0, torch.zeros(8, dtype=torch.bool, device=device))
+    assert loss.item() == 0.0 and (grad == 0).all()
+
+
+@pytest.mark.parametrize("device", CPU_GPU)
+def test_distill_whole_row_in_the_record(device):
+    need(device)
+    x = make_logits(1, 3, 200, torch.float32, device)
+    values, indices, lse = make_record(x, 200, 1.0)
+    check_distill(x, values, indices, lse)
+
+
+@pytest.mark.parametrize("device", CPU_GPU)
+def test_distill_rest_that_underflows(device):
+    """The student gives the record everything: q outside is e^-200, and the
+    rest's term is still its logarithm."""
+    need(device)
+    x = torch.full((1, 2, 500), -200.0, device=device)
+    x[..., :3] = 0.0
+    values = torch.zeros(1, 2, 3, device=device)
+    indices = torch.arange(3, device=device).expand(1, 2, 3)
+    lse = torch.full((1, 2), math.log(4.0), device=device)
+    loss, grad = check_distill(x, values, indices, lse)
+    assert loss.item() > 40.0
+    assert abs(grad[..., 3:].sum().item() / -0.25 - 1) < 1e-4
+
+
+@pytest.mark.parametrize("device", CPU_GPU)
+def test_distill_index_outside_is_nan(device):
+    need(device)
+    x = make_logits(1, 3, 64, torch.float32, device)
+    values, indices, _ = make_record(x, 4, 1.0)
+    indices[0, 1, 2] = 64
+    x.requires_grad_(True)
+    loss = distill_loss(x, values, indices, reduction="none")
+    assert torch.isnan(loss[0, 1]) and torch.isfinite(loss[0, [0, 2]]).all()
+    grad, = torch.autograd.grad(loss.sum(), x)
+    assert torch.isfinite(grad[0, [0, 2]]).all() and torch.isnan(grad[0, 1]).all()
+
+
+# ------------------------------------------------------------------ preference
+def preference_oracle(logits, targets, ref, beta, eps, ignore):
+    N = logits.shape[0] // 2
+    lq = softmax64(logits)
+    tg = targets.cpu().long()
+    keep = tg != ignore
+    lp = torch.where(keep, lq.gather(-1, tg.clamp_min(0)[..., None])[..., 0], 0.0)
+    r = beta * (lp.sum(-1) - ref.cpu().double())
+    z = r[:N] - r[N:]
+    loss = -((1 - eps) * torch.nn.functional.logsigmoid(z) + eps * torch.nn.functional.logsigmoid(-z))
+    by_z = torch.sigmoid(z) - (1 - eps)
+    a = beta * torch.cat([by_z, -by_z])[:, None] * keep
+    one = torch.zeros_like(lq).scatter_(-1, tg.clamp_min(0)[..., None], 1.0)
+    grad = torch.where(a[..., None] != 0, a[..., None] * (one - lq.exp()), 0.0)
+    return loss, r, grad, a, lq.exp()
+
+
+def check_preference(logits, targets, ref, beta=0.1, eps=0.0, ignore=-100, reduction="mean", up=None):
+    x = logits.detach().requires_grad_(True) if logits.is_leaf else logits
+    out = preference_loss(x, targets, ref, beta=beta, label_smoothing=eps, ignore_index=ignore,
+                          reduction=reduction)
+    rows, r, grad, a, q = preference_oracle(logits, targets, ref, beta, eps, ignore)
+    N, T = len(rows), targets.shape[1]
+    want = {"mean": rows.mean(), "sum": rows.sum(), "none": rows}[reduction]
+    lim = 2 * beta * T * LP
+    torch.testing.assert_close(out.loss.detach().cpu().double(), want, rtol=2.0 ** -22,
+                               atol=lim * (N if reduction == "sum" else 1))
+    rewards = torch.cat([out.chosen_rewards, out.rejected_rewards])
+    torch.testing.assert_close(rewards.cpu().double(), r, rtol=2.0 ** -22, atol=lim)
+    assert not rewards.requires_grad
+    up = torch.ones_like(out.loss) if up is None else up
+    got, = torch.autograd.grad(out.loss, x, up)
+    u = up.cpu().double()
+    each = u.repeat(2)[:, None] if reduction == "none" else u / (N if reduction == "mean" else 1)
+    # the coefficient moves by lim of z's error beside the rounding of q
+    slack = (lim / GRAD + 1) if lim > GRAD else 2
+    check_grad(got, grad * each[..., None], a * each * slack, q + (q * 0 + grad.abs() / a.abs().clamp_min(1e-300)[..., None]) * (a != 0)[..., None])
+    assert (got.cpu()[(targets == ignore).cpu()] == 0).all()
+    return out, got
+
+
+def make_pairs(N, T, V, device, seed=2):
+    g = torch.Generator().manual_seed(seed)
+    targets = torch.randint(0, V, (2 * N, T), generator=g)
+    lengths = torch.randint(0, T + 1, (2 * N, 1), generator=g)
+    targets = torch.where(torch.arange(T)[None] < lengths, targets, -100)
+    ref = torch.randn(2 * N, generator=g) * 5 - 10.0 * (targets >= 0).sum(-1)
+    return targets.to(device), ref.to(device)
+
+
+@pytest.mark.parametrize("device", CPU_GPU)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", SHAPES)
+def test_preference(device, dtype, shape):
+    need(device)
+    B, T, V = shape
+    x = make_logits(2 * B, T, V, dtype, device)
+    targets, ref = make_pairs(B, T, V, device)
+    scale = 512.0 if dtype == torch.float16 else 1.0
+    check_preference(x, targets, ref, eps=0.1 if B > 1 else 0.0,
+                     up=torch.tensor(scale, device=device))
+
+
+@pytest.mark.parametrize("device", CPU_GPU)
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+def test_preference_reductions_and_layouts(device, reduction):
+    need(device)
+    x = make_logits(6, 6, 515, torch.float32, device)
+    targets, ref = make_pairs(3, 5, 512, device)
+    up = torch.tensor([0.5, -2.0, 3.0] if reduction == "none" else 1.75, device=device)
+    for view in (x[:, :-1, :], x[:, 1:, :512], x[:, :5, 3:],
+                 x[:, 1:].transpose(0, 1).contiguous().transpose(0, 1)):
+        check_preference(view, targets, ref.double(), reduction=reduction, up=up)
+    # another ignored index, whose token is a real one; int32 targets
+    targets[:, 0] = 7
+    check_preference(x[:, 1:], targets.clamp_min(0).int(), ref, ignore=7, reduction=reduction, up=up)
+
+
+@pytest.mark.parametrize("device", CPU_GPU)
+def test_preference_masked_rows_hold_anything(device):
+    need(device)
+    x = make_logits(4, 5, 130, torch.float32, device)
+    targets, ref = make_pairs(2, 5, 130, device, seed=11)
+    targets[0] = -100  # an answer of no tokens
+    want, grad = check_preference(x, targets, ref)
+    bad = x.clone()
+    bad[targets == -100] = float("nan")
+    bad.requires_grad_(True)
+    got = preference_loss(bad, targets, ref)
+    assert torch.equal(got.loss.detach(), want.loss.detach())
+    g, = torch.autograd.grad(got.loss, bad)
+    assert torch.equal(g, grad)
+
+
+@pytest.mark.parametrize("device", CPU_GPU)
+def test_preference_far_margins(device):
+    """sigmoid and its logarithm far out: no overflow, no 0 * inf."""
+    need(device)
+    x = make_logits(4, 3, 64, torch.float32, device)
+    targets = torch.zeros(4, 3, dtype=torch.int64, device=device)
+    ref = torch.tensor([-1e6, 1e6, 0.0, 0.0], device=device)
+    check_preference(x, targets, ref, reduction="none")
+
+
+@pytest.mark.parametrize("device", CPU_GPU)
+def test_preference_target_outside_is_nan(device):
+    need(device)
+    x = make_logits(4, 3, 64, torch.float32, device).requires_grad_(True)
+    targets = torch.zeros(4, 3, dtype=torch.int64, device=device)
+    targets[1, 2] = 64
+    targets[2, 0] = -7
+    out = preference_loss(x[:2], targets[:2], torch.zeros(2, device=device), reduction="none")
+    assert torch.isnan(out.loss).all()
+    out = preference_loss(x[2:], targets[2:], torch.zeros(2, device=device), reduction="none")
+    assert torch.isnan(out.loss).all()
+
+
+# ---------------------------------------------------------------------- policy
+def policy_oracle(logits, actions, old, adv, ref, mask, low, high, coef):
+    lq = softmax64(logits)
+    act = actions.cpu().long()
+    live = torch.ones(act.shape, dtype=torch.bool) if mask is None else mask.cpu()
+    lp = torch.where(live, lq.gather(-1, act[..., None])[..., 0], 0.0)
+    A = torch.where(live, adv.cpu(), 0).double()
+    ratio = (lp - torch.where(live, old.cpu(), 0).double()).exp()
+    held = ratio.clamp(1 - low, 1 + high)
+    loss = -torch.minimum(ratio * A, held * A)
+    moves = torch.where(A > 0, ratio <= 1 + high, ratio >= 1 - low)
+    by_lp = torch.where(moves, -A * ratio, 0.0)
+    kl = torch.zeros_like(lp)
+    if ref is not None:
+        d = torch.where(live, ref.cpu(), 0).double() - lp
+        kl = torch.expm1(d) - d
+        loss = loss + coef * kl
+        by_lp = by_lp - coef * torch.expm1(d)
+    by_lp = by_lp * live
+    one = torch.zeros_like(lq).scatter_(-1, act[..., None], 1.0)
+    grad = torch.where(by_lp[..., None] != 0, by_lp[..., None] * (one - lq.exp()), 0.0)
+    return loss * live, lp, kl * live, grad, by_lp, lq.exp(), live
+
+
+def make_rollout(logits, seed=4, spread=0.3):
+    """Old log-probabilities that keep 1e-3 from the borders of the clip."""
+    g = torch.Generator().manual_seed(seed)
+    rows = logits.shape[:-1]
+    actions = torch.randint(0, logits.shape[-1], rows, generator=g)
+    lp = softmax64(logits).gather(-1, actions[..., None])[..., 0]
+    moved = torch.randn(rows, generator=g).double() * spread
+    for border in (math.log(1.2), math.log(0.8), math.log(1.3)):
+        moved = torch.where((moved - border).abs() < 1e-3, moved + 4e-3, moved)
+    adv = torch.randn(rows, generator=g)
+    ref = (lp + torch.randn(rows, generator=g) * 0.3).float()
+    return [a.to(logits.device) for a in (actions, (lp - moved).float(), adv, ref)]
+
+
+def check_policy(logits, actions, old, adv, ref, mask=None, low=0.2, high=0.2, coef=0.05,
+                 reduction="mean", up=None):
+    x = logits.detach().requires_grad_(True) if logits.is_leaf else logits
+    out = policy_loss(x, actions, old, adv, ref, mask=mask, clip_low=low, clip_high=high,
+                      kl_coef=coef, reduction=reduction)
+    rows, lp, kl, grad, by_lp, q, live = policy_oracle(logits, actions, old, adv, ref, mask,
+                                                       low, high, coef)
+    n = max(int(live.sum()), 1)
+    want = {"mean": rows.sum() / n, "sum": rows.sum(), "none": rows}[reduction]
+    # a ratio of at most e^2 * |A| <= 5 and an exp(d) of at most e^2: 50 LP
+    lim = 50 * LP * (n if reduction == "sum" else 1)
+    torch.testing.assert_close(out.loss.detach().cpu().double(), want, rtol=2.0 ** -22, atol=lim)
+    torch.testing.assert_close(out.logps.cpu().double(), lp, rtol=2.0 ** -23, atol=LP)
+    torch.testing.assert_close(out.kl.cpu().double(), kl, rtol=2.0 ** -22, atol=10 * LP)
+    assert not out.logps.requires_grad and not out.kl.requires_grad
+    up = torch.ones_like(out.loss) if up is None else up
+    got, = torch.autograd.grad(out.loss, x, up)
+    u = up.cpu().double()
+    each = u if reduction == "none" else u / (n if reduction == "mean" else 1)
+    each = each * torch.ones_like(by_lp)
+    # the terms of by_lp may cancel: its error is that of the larger ones
+    big = (by_lp.abs() + (adv.cpu().double().abs() * 2 + coef * 3) * live) * each.abs()
+    check_grad(got, grad * each[..., None], big, q + (1 - q) * (grad != 0))
+    assert (got.cpu()[by_lp == 0] == 0).all()
+    return out, got
+
+
+@pytest.mark.parametrize("device", CPU_GPU)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", SHAPES)
+def test_policy(device, dtype, shape):
+    need(device)
+    B, T, V = shape
+    x = make_logits(B, T, V, dtype, device)
+    actions, old, adv, ref = make_rollout(x)
+    mask = None
+    if B > 1:
+        mask = (torch.arange(T)[None] < torch.randint(1, T + 1, (B, 1),
+                                                      generator=torch.Generator().manual_seed(5)))
+        mask = mask.to(device)
+    scale = 512.0 if dtype == torch.float16 else 1.0
+    check_policy(x, actions, old, adv, ref if T > 1 else None, mask, coef=0.05 if T > 1 else 0.0,
+                 up=torch.tensor(scale, device=device))
+
+
+@pytest.mark.parametrize("device", CPU_GPU)
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+def test_policy_reductions_and_layouts(device, reduction):
+    need(device)
+    x = make_logits(3, 7, 515, torch.float32, device)
+    for view in (x[:, :-1], x[:, 1:, :512], x[:, :6, 3:], x[0, 1:], x[1, 2],
+                 x.transpose(0, 1)[1:], x[:, :6].reshape(3, 2, 3, 515)):
+        actions, old, adv, ref = make_rollout(view)
+        up = torch.randn(adv.shape if reduction == "none" else (),
+                         generator=torch.Generator().manual_seed(1)).to(device)
+        check_policy(view, actions.int(), old, adv, ref, low=0.2, high=0.3, reduction=reduction,
+                     up=up)
+
+
+@pytest.mark.parametrize("device", CPU_GPU)
+def test_policy_masks(device):
+    need(device)
+    x = make_logits(2, 5, 130, torch.float32, device)
+    actions, old, adv, ref = make_rollout(x)
+    mask = torch.tensor([[1, 1, 0, 0, 1], [0, 0, 0, 0, 0]], dtype=torch.bool, device=device)
+    want, grad = check_policy(x, actions, old, adv, ref, mask)
+    for t in (x, old, adv, ref):
+        t[~mask] = float("nan")
+    actions[~mask] = -100
+    x.requires_grad_(True)
+    got = policy_loss(x, actions, old, adv, ref, mask=mask, kl_coef=0.05)
+    g, = torch.autograd.grad(got.loss, x)
+    assert torch.equal(got.loss.detach(), want.loss.detach()) and torch.equal(g, grad)
+    assert torch.equal(got.kl, want.kl) and torch.equal(got.logps, want.logps)
+    none = policy_loss(x, actions, old, adv, ref, mask=torch.zeros_like(mask), kl_coef=0.05)
+    assert none.loss.item() == 0.0
+    g, = torch.autograd.grad(none.loss, x)
+    assert (g == 0).all()
+
+
+@pytest.mark.parametrize("device", CPU_GPU)
+@pytest.mark.parametrize("dtype", TYPES)
+def test_masked_logits(device, dtype):
+    """-inf (a padded head) and the type's lowest value in a row: no gradient
+    there, none lost elsewhere; a row of the lowest value alone is uniform."""
+    need(device)
+    x = make_logits(2, 3, 600, dtype, device)
+    x[..., 500:] = float("-inf")
+    x[1, ..., 400:500] = torch.finfo(dtype).min
+    x[1, 2] = torch.finfo(dtype).min
+    actions = torch.randint(0, 400, (2, 3), generator=torch.Generator().manual_seed(8)).to(device)
+    old = softmax64(x).gather(-1, actions.cpu()[..., None])[..., 0].float().to(device)
+    adv = torch.ones(2, 3, device=device)
+    _, grad = check_policy(x, actions, old, adv, None, coef=0.0)
+    assert (grad[0, :, 500:] == 0).all()
+
+
+@pytest.mark.parametrize("device", CPU_GPU)
+def test_policy_action_outside_and_bad_logits_are_nan(device):
+    need(device)
+    x = make_logits(1, 6, 64, torch.float32, device)
+    x[0, 2, 5] = float("nan")
+    x[0, 3, 5] = float("inf")
+    x[0, 4] = float("-inf")
+    x.requires_grad_(True)
+    actions = torch.tensor([[64, -1, 3, 3, 3, 3]], device=device)
+    zero = torch.zeros(1, 6, device=device)
+    out = policy_loss(x, actions, zero, zero + 1, reduction="none")
+    assert torch.isnan(out.loss[0, :5]).all() and torch.isfinite(out.loss[0, 5])
+    g, = torch.autograd.grad(out.loss.sum(), x)
+    assert torch.isnan(g[0, :5]).any(-1).all() and torch.isfinite(g[0, 5]).all()
+
+
+# ------------------------------------------------------ gradients by differences
+def test_gradients_by_differences():
+    """The CPU definitions that the kernels are held to, in float64."""
+    x = make_logits(4, 3, 11, torch.float64, "cpu", scale=1.0).requires_grad_(True)
+    values, indices, lse = make_record(x, 4, 1.5)
+    values = values.detach()
+    for record in ((values, indices), (values, indices, lse.double())):
+        assert torch.autograd.gradcheck(
+            lambda y: distill_loss(y, *record, temperature=1.5), (x,))
+    targets, ref = make_pairs(2, 3, 11, "cpu")
+    assert torch.autograd.gradcheck(lambda y: preference_loss(
+        y, targets, ref, label_smoothing=0.1).loss, (x,))
+    actions, old, adv, kref = make_rollout(x)
+    assert torch.autograd.gradcheck(lambda y: policy_loss(
+        y, actions, old, adv, kref, kl_coef=0.1).loss, (x,))
+
+
+@pytest.mark.gpu
+def test_kernel_gradients_by_differences():
+    """The kernels' own loss moves as their own gradient says. Central
+    differences of step h along a direction: off by h^2 times a third
+    derivative (< 1) and by two losses' rounding, 4 LP, over 2 h."""
+    need("cuda")
+    h = 0.05
+    x = make_logits(4, 3, 203, torch.float32, "cuda", scale=1.0)
+    d = make_logits(4, 3, 203, torch.float32, "cuda", seed=9, scale=1.0)
+    d /= d.norm()
+    values, indices, lse = make_record(x, 7, 1.0)
+    targets, ref = make_pairs(2, 3, 203, "cuda")
+    actions, old, adv, kref = make_rollout(x, spread=0.05)
+    for fn in (lambda y: distill_loss(y, values, indices),
+               lambda y: distill_loss(y, values, indices, lse),
+               lambda y: preference_loss(y, targets, ref).loss,
+               lambda y: policy_loss(y, actions, old, adv, kref, kl_coef=0.1, clip_low=0.9,
+                                     clip_high=9.0).loss):
+        y = x.clone().requires_grad_(True)
+        g, = torch.autograd.grad(fn(y), y)
+        slope = (g * d).sum().item()
+        with torch.no_grad():
+            moved = (fn(x + h * d).item() - fn(x - h * d).item()) / (2 * h)
+        assert abs(moved - slope) <= h * h + 4 * LP / (2 * h), (moved, slope)
+
+
+# -------------------------------------------------------------------- refusals
+@pytest.mark.parametrize("device", CPU_GPU)
+def test_refusals(device):
+    need(device)
+    x = make_logits(2, 3, 40, torch.float32, device)
+    values, indices, lse = make_record(x, 4, 1.0)
+    targets = torch.zeros(2, 3, dtype=torch.int64, device=device)
+    rows = torch.zeros(2, 3, device=device)
+    ref = torch.zeros(2, device=device)
+    bad = [
+        lambda: topk_logits(x, 0), lambda: topk_logits(x, 41),
+        lambda: topk_logits(x.int(), 2), lambda: topk_logits(x, 2, 0.0),
+        lambda: topk_logits(make_logits(1, 1, 400, torch.float32, device), 257),
+        lambda: topk_logits(torch.zeros((), device=device), 1),
+        lambda: topk_logits(x, 2, float("nan")),
+        lambda: distill_loss(x, values, indices, temperature=-1.0),
+        lambda: distill_loss(x, values, indices, reduction="max"),
+        lambda: distill_loss(x, values[:, :2], indices),
+        lambda: distill_loss(x, values, indices[..., :3]),
+        lambda: distill_loss(x, values, indices.float()),
+        lambda: distill_loss(x, indices, indices),
+        lambda: distill_loss(x, values, indices, lse[:1]),
+        lambda: distill_loss(x, values, indices, mask=rows),
+        lambda: distill_loss(x, values, indices, mask=torch.ones(3, dtype=torch.bool, device=device)),
+        lambda: distill_loss(x, values.clone().requires_grad_(True), indices),
+        lambda: distill_loss(x, values[..., :0], indices[..., :0]),
+        lambda: distill_loss(x, torch.zeros(2, 3, 257, device=device),
+                             torch.zeros(2, 3, 257, dtype=torch.int64, device=device)),
+        lambda: preference_loss(x[0], targets[0], ref),
+        lambda: preference_loss(x[:1], targets[:1], ref[:1]),
+        lambda: preference_loss(x, targets[:, :2], ref),
+        lambda: preference_loss(x, targets.float(), ref),
+        lambda: preference_loss(x, targets, ref[:1]),
+        lambda: preference_loss(x, targets, ref.long()),
+        lambda: preference_loss(x, targets, ref, beta=0.0),
+        lambda: preference_loss(x, targets, ref, label_smoothing=0.5),
+        lambda: preference_loss(x, targets, ref.clone().requires_grad_(True)),
+        lambda: preference_loss(x[:, :0], targets[:, :0], ref),
+        lambda: policy_loss(x, targets, rows[:1], rows),
+        lambda: policy_loss(x, targets.bool(), rows, rows),
+        lambda: policy_loss(x, targets, rows, rows, kl_coef=0.1),
+        lambda: policy_loss(x, targets, rows, rows, clip_low=1.0),
+        lambda: policy_loss(x, targets, rows, rows, clip_high=-0.1),
+        lambda: policy_loss(x, targets, rows, rows, rows, kl_coef=-1.0),
+        lambda: policy_loss(x, targets, rows, rows.clone().requires_grad_(True)),
+        lambda: policy_loss(x, targets, rows, rows, mask=targets),
+    ]
+    if device == "cuda":
+        bad += [lambda: topk_logits(x.double(), 2),
+                lambda: policy_loss(x, targets.cpu(), rows, rows),
+                lambda: preference_loss(x, targets, ref.cpu()),
+                lambda: distill_loss(x, values.cpu(), indices)]
+    for i, call in enumerate(bad):
+        with pytest.raises(ValueError):
+            call()
+            pytest.fail(f"call {i} was not refused")
+
+
+@pytest.mark.parametrize("device", CPU_GPU)
+def test_no_rows(device):
+    need(device)
+    x = torch.zeros(0, 3, 40, device=device, requires_grad=True)
+    rows = torch.zeros(0, 3, device=device)
+    ids = torch.zeros(0, 3, dtype=torch.int64, device=device)
+    record = torch.zeros(0, 3, 2, device=device), torch.zeros(0, 3, 2, dtype=torch.int64, device=device)
+    for loss in (distill_loss(x, *record), policy_loss(x, ids, rows, rows).loss,
+                 policy_loss(x, ids, rows, rows, reduction="sum").loss):
+        assert loss.item() == 0.0
+        g, = torch.autograd.grad(loss, x)
+        assert g.shape == x.shape
+    assert distill_loss(x, *record, reduction="none").shape == (0, 3)
+
+
+# ----------------------------------------------------- streams, graphs, memory
+def all_losses(x, pairs, rollout, record, lse):
+    return (distill_loss(x, *record, lse, temperature=2.0),
+            preference_loss(x, *pairs).loss,
+            policy_loss(x, *rollout, kl_coef=0.05).loss)
+
+
+@pytest.mark.gpu
+def test_same_bits_again_and_backward_twice():
+    need("cuda")
+    x = make_logits(4, 37, 5003, torch.bfloat16, "cuda").requires_grad_(True)
+    values, indices, lse = make_record(x, 9, 2.0)
+    pairs, rollout = make_pairs(2, 37, 5003, "cuda"), make_rollout(x)
+    first = None
+    for _ in range(3):
+        losses = all_losses(x, pairs, rollout, (values, indices), lse)
+        grads = [torch.autograd.grad(l, x, retain_graph=True)[0] for l in losses]
+        again = [torch.autograd.grad(l, x)[0] for l in losses]
+        now = [l.detach() for l in losses] + grads
+        assert all(torch.equal(a, b) for a, b in zip(grads, again))
+        assert first is None or all(torch.equal(a, b) for a, b in zip(first, now))
+        first = now
+
+
+@pytest.mark.gpu
+def test_gradient_reaches_views_and_accumulates():
+    need("cuda")
+    base = make_logits(4, 6, 515, torch.float32, "cuda").requires_grad_(True)
+    targets, ref = make_pairs(2, 5, 512, "cuda")
+    for _ in range(2):
+        preference_loss(base[:, :-1, :512], targets, ref).loss.backward()
+    _, _, grad, _, _ = preference_oracle(base[:, :-1, :512], targets, ref, 0.1, 0.0, -100)
+    assert (base.grad[:, -1] == 0).all() and (base.grad[..., 512:] == 0).all()
+    torch.testing.assert_close(base.grad[:, :-1, :512].cpu().double(), grad, rtol=1e-3, atol=1e-6)
+
+
+@pytest.mark.gpu
+def test_second_derivative_is_refused():
+    need("cuda")
+    x = make_logits(1, 3, 64, torch.float32, "cuda").requires_grad_(True)
+    values, indices, _ = make_record(x, 4, 1.0)
+    loss = distill_loss(x, values, indices)
+    with pytest.raises(RuntimeError, match="second derivative"):
+        torch.autograd.grad(loss, x, create_graph=True)
+
+
+@pytest.mark.gpu
+def test_another_stream():
+    need("cuda")
+    x = make_logits(4, 64, 30522, torch.bfloat16, "cuda").requires_grad_(True)
+    values, indices, lse = make_record(x, 9, 2.0)
+    pairs, rollout = make_pairs(2, 64, 30522, "cuda"), make_rollout(x)
+    want = all_losses(x, pairs, rollout, (values, indices), lse)
+    want = [(l.detach(), torch.autograd.grad(l, x)[0]) for l in want]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = all_losses(x, pairs, rollout, (values, indices), lse)
+        got = [(l.detach(), torch.autograd.grad(l, x)[0]) for l in got]
+        top = topk_logits(x, 5)
+    side.synchronize()
+    for (a, b), (c, d) in zip(want, got):
+        assert torch.equal(a, c) and torch.equal(b, d)
+    assert torch.equal(top.indices, topk_logits(x, 5).indices)
+
+
+@pytest.mark.gpu
+def test_two_captured_graphs():
+    """Forward and backward in two graphs that share nothing, replayed in turn
+    on new inputs with eager calls between."""
+    need("cuda")
+    graphs, static = [], []
+    for seed in (0, 1):
+        x = make_logits(4, 21, 4099, torch.bfloat16, "cuda", seed=seed).requires_grad_(True)
+        values, indices, lse = make_record(x, 9, 2.0)
+        pairs, rollout = make_pairs(2, 21, 4099, "cuda"), make_rollout(x)
+
+        def step(x=x, pairs=pairs, rollout=rollout, record=(values, indices), lse=lse):
+            losses = all_losses(x, pairs, rollout, record, lse)
+            grads = [torch.autograd.grad(l, x)[0] for l in losses]
+            return [l.detach() for l in losses] + grads + list(topk_logits(x.detach(), 5))
+
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step()
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step()
+        graphs.append((graph, out, step))
+        static.append(x)
+    for turn in range(4):
+        for (graph, out, step), x in zip(graphs, static):
+            with torch.no_grad():
+                x.copy_(make_logits(4, 21, 4099, torch.bfloat16, "cuda", seed=10 + turn))
+            graph.replay()
+            torch.cuda.synchronize()
+            got = [o.clone() for o in out]
+            assert all(torch.equal(a, b) for a, b in zip(got, step()))
+            torch.cuda.synchronize()
+
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits():
+    """Rows behind 2^31 logits: 4.6 GB of them, with the last rows checked."""
+    need("cuda")
+    T, V = 18000, 128256
+    x = torch.empty(1, T, V, dtype=torch.bfloat16, device="cuda").normal_()
+    x.requires_grad_(True)
+    actions = torch.randint(0, V, (1, T), device="cuda")
+    old = torch.full((1, T), -12.0, device="cuda")
+    out = policy_loss(x, actions, old, torch.ones(1, T, device="cuda"), clip_high=1e6,
+                      reduction="sum")
+    grad, = torch.autograd.grad(out.loss, x)
+    top = topk_logits(x, 3)
+    for r in (0, 9000, 16744, 17999):
+        row = x.detach()[0, r].double()
+        lq = torch.log_softmax(row, -1)
+        lp = lq[actions[0, r]]
+        assert abs(out.logps[0, r].item() - lp.item()) <= LP + 2.0 ** -20
+        a = (lp + 12.0).exp()
+        want = a * lq.exp()
+        want[actions[0, r]] -= a
+        check_grad(grad[0, r], want, a, lq.exp().cpu())
+        assert torch.equal(top.values[0, r], row.topk(3).values.bfloat16())
+
+
+# ------------------------------------------------------------- used together
+@pytest.mark.parametrize("device", CPU_GPU)
+@pytest.mark.parametrize("tail", [False, True])
+def test_station_learns_from_a_record(device, tail):
+    """A teacher's record of its own answers pulls a student's logits to the
+    teacher's: the gradient vanishes at the teacher and points there elsewhere."""
+    need(device)
+    g = torch.Generator().manual_seed(0)
+    h = torch.randn(2, 6, 16, generator=g).to(device)
+    wt = torch.randn(64, 16, generator=g).to(device)
+    teacher = h @ wt.t()
+    record = topk_logits(teacher, 64, 2.0)
+    lse = record.logsumexp if tail else None
+    w = wt.clone().requires_grad_(True)
+    loss = distill_loss(h @ w.t(), record.values, record.indices, lse, temperature=2.0)
+    at, = torch.autograd.grad(loss, w)
+    # KL at the teacher is 0 up to LP; the gradient up to LP times |h| < 6
+    assert abs(loss.item()) <= 8 * LP and at.abs().max().item() <= 12 * LP
+    w = (wt * 0.5).requires_grad_(True)
+    record = topk_logits(teacher, 8, 2.0)
+    lse = record.logsumexp if tail else None
+    loss = distill_loss(h @ w.t(), record.values, record.indices, lse, temperature=2.0)
+    grad, = torch.autograd.grad(loss, w)
+    with torch.no_grad():
+        down = distill_loss(h @ (w - 1e-2 * grad).t(), record.values, record.indices, lse,
+                            temperature=2.0)
+    slope = (grad * grad).sum().item()
+    assert down.item() < loss.item() - 0.5 * 1e-2 * slope

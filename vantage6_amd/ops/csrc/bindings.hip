@@ -4,6 +4,7 @@
 #include <hip/hip_runtime.h>
 
 #include "common.h"
+#include "lm_loss.h"
 
 // kernels defined in sibling TUs
 extern "C" __global__ void fused_sgd_kernel(short*, float*, const short*, float*,
@@ -552,6 +553,323 @@ torch::Tensor ce_bwd(torch::Tensor x, torch::Tensor t, torch::Tensor lse,
                      dlv.data_ptr<float>(), (short*)dx.data_ptr(), V,
                      ignore_index);
   return dx;
+}
+
+// ------------------------------------------------ losses over LM logits
+// (lm_loss.hip). Logits are [V], [T, V] or [B, T, V] with any strides over the
+// rows; everything given per row has the shape of the rows.
+static int lm_type(const torch::Tensor& t, const char* what) {
+  switch (t.scalar_type()) {
+    case torch::kBFloat16: return LM_BF16;
+    case torch::kHalf: return LM_FP16;
+    case torch::kFloat32: return LM_FP32;
+    default: TORCH_CHECK(false, what, " must be bf16, fp16 or fp32");
+  }
+}
+
+static LmRows lm_rows(const torch::Tensor& x, double temperature) {
+  TORCH_CHECK(x.is_cuda(), "logits must be a HIP tensor");
+  TORCH_CHECK(x.dim() >= 1 && x.dim() <= 3, "logits must be [V], [T, V] or [B, T, V]");
+  const int64_t d = x.dim(), V = x.size(d - 1);
+  const int64_t T = d > 1 ? x.size(d - 2) : 1, B = d > 2 ? x.size(0) : 1;
+  TORCH_CHECK(V >= 1 && V < (1LL << 30), "logits: unsupported vocabulary size");
+  TORCH_CHECK(V == 1 || x.stride(d - 1) == 1, "logits of a row must be contiguous");
+  TORCH_CHECK(B * T < (1LL << 22), "logits: at most 4194303 rows a call");
+  LmRows in;
+  in.x = x.data_ptr();
+  in.sb = d > 2 ? x.stride(0) : 0;
+  in.st = d > 1 ? x.stride(d - 2) : 0;
+  in.T = (int)T;
+  in.R = (int)(B * T);
+  in.V = (int)V;
+  in.type = lm_type(x, "logits");
+  const double c = 1.4426950408889634074 / temperature;
+  in.c = (float)c;
+  in.c_lo = (float)(c - in.c);
+  return in;
+}
+
+static void lm_check_grid(const LmRows& in, int splits) {
+  // a grid counts its threads in 32 bits
+  TORCH_CHECK((long long)in.R * (splits + 1) < (1LL << 24),
+              "logits: too many rows for one call at this vocabulary size");
+}
+
+// contiguous, of one element per row, on the logits' device
+static torch::Tensor lm_per_row(const torch::Tensor& t, const torch::Tensor& x,
+                                torch::ScalarType type, const char* what) {
+  TORCH_CHECK(t.device() == x.device(), what, " must be on the logits' device");
+  TORCH_CHECK(t.sizes() == x.sizes().slice(0, x.dim() - 1), what,
+              " must have the shape of the logits' rows");
+  return t.to(type).contiguous();
+}
+
+static const void* lm_ptr(const c10::optional<torch::Tensor>& t) {
+  return t.has_value() ? t->data_ptr() : nullptr;
+}
+
+// keep: {stat [R] of 4, coef [R], inv, p [R, K]} floats
+static torch::Tensor lm_keep(const torch::Tensor& x, const LmRows& in, int K,
+                             LmKeep* kp) {
+  const long long R = in.R;
+  auto keep = torch::empty({R * (5 + K) + 1},
+                           x.options().dtype(torch::kFloat32).requires_grad(false));
+  float* f = keep.data_ptr<float>();
+  *kp = {(LmStat*)f, f + 4 * R, f + 5 * R, K ? f + 5 * R + 1 : nullptr};
+  return keep;
+}
+
+// the bytes behind a forward pass's workspaces
+static torch::Tensor lm_work(const torch::Tensor& x, const LmRows& in, bool rest,
+                             bool record, int blocks, LmWork* w) {
+  const long long R = in.R;
+  w->splits = lm_stats_splits(in);
+  lm_check_grid(in, w->splits);
+  const long long part = 8 * R * w->splits;
+  const long long n_rec = record ? 32 * R : 0, n_b = 16LL * blocks;
+  auto ws = torch::empty({n_rec + n_b + part * (rest ? 2 : 1) + 16},
+                         x.options().dtype(torch::kUInt8).requires_grad(false));
+  char* at = (char*)ws.data_ptr();
+  w->rec = record ? (double4*)at : nullptr;
+  w->bpart = (double2*)(at + n_rec);
+  w->part = (float2*)(at + n_rec + n_b);
+  w->part_top = rest ? (float2*)(at + n_rec + n_b + part) : nullptr;
+  w->counter = (int*)(at + n_rec + n_b + part * (rest ? 2 : 1));
+  return ws;
+}
+
+static torch::Tensor lm_loss_out(const torch::Tensor& x, at::IntArrayRef each,
+                                 int64_t reduction, const LmKeep& kp, LmOut* o) {
+  TORCH_CHECK(reduction >= LM_MEAN && reduction <= LM_NONE, "unknown reduction");
+  auto opt = x.options().dtype(torch::kFloat32).requires_grad(false);
+  auto loss = reduction == LM_NONE ? torch::empty(each, opt) : torch::empty({}, opt);
+  *o = {loss.data_ptr<float>(), kp.inv, (int)reduction};
+  return loss;
+}
+
+static void lm_set_idx(LmPlaces* pl, const torch::Tensor& idx) {
+  TORCH_CHECK(idx.scalar_type() == torch::kLong || idx.scalar_type() == torch::kInt,
+              "indices must be int64 or int32");
+  pl->idx = idx.data_ptr();
+  pl->idx64 = idx.scalar_type() == torch::kLong;
+}
+
+std::vector<torch::Tensor> lm_topk_fwd(torch::Tensor x, int64_t k,
+                                       double temperature) {
+  LmRows in = lm_rows(x, temperature);
+  TORCH_CHECK(k >= 1 && k <= kLmMostK && k <= in.V, "topk: k out of range");
+  c10::DeviceGuard guard(x.device());
+  auto opt = x.options().requires_grad(false);
+  auto sizes = x.sizes().vec();
+  sizes.back() = k;
+  auto values = torch::empty(sizes, opt);
+  auto idx = torch::empty(sizes, opt.dtype(torch::kLong));
+  sizes.pop_back();
+  auto lse = torch::empty(sizes, opt.dtype(torch::kFloat32));
+  if (in.R)
+    lm_topk(in, (float)temperature, (int)k, values.data_ptr(),
+            (long long*)idx.data_ptr(), lse.data_ptr<float>(), cur_stream());
+  return {values, idx, lse};
+}
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+// d(loss)/d(logits) from what a forward pass kept: saved {logits, idx, keep}
+static torch::Tensor lm_backward(AutogradContext* ctx, const torch::Tensor& grad,
+                                 int64_t per, int64_t K, double temperature) {
+  TORCH_CHECK(!at::GradMode::is_enabled(),
+              "losses over logits have no second derivative");
+  const auto saved = ctx->get_saved_variables();
+  const torch::Tensor &x = saved[0], &idx = saved[1], &keep = saved[2];
+  LmRows in = lm_rows(x, temperature);
+  c10::DeviceGuard guard(x.device());
+  const long long R = in.R;
+  const int64_t pairs = per == LM_UP_PAIR ? x.size(0) / 2 : 1;
+  auto dx = torch::empty(x.sizes(), x.options().requires_grad(false));
+  if (!R) return dx;
+  auto up = grad.to(torch::kFloat32).contiguous();
+  lm_check_grid(in, lm_grad_splits(in));
+  float* f = keep.data_ptr<float>();
+  LmKeep kp{(LmStat*)f, f + 4 * R, f + 5 * R, K ? f + 5 * R + 1 : nullptr};
+  LmPlaces pl{};
+  lm_set_idx(&pl, idx);
+  pl.K = K ? (int)K : 1;
+  LmUp u{up.data_ptr<float>(), (int)per, (int)pairs};
+  lm_grad(in, pl, kp, u, dx.data_ptr(), cur_stream());
+  return dx;
+}
+
+struct LmDistillFn : public torch::autograd::Function<LmDistillFn> {
+  static torch::Tensor forward(AutogradContext* ctx, torch::Tensor x,
+                               torch::Tensor values, torch::Tensor idx,
+                               c10::optional<torch::Tensor> lse,
+                               double temperature,
+                               c10::optional<torch::Tensor> mask,
+                               int64_t reduction) {
+    LmRows in = lm_rows(x, temperature);
+    const int64_t K = idx.dim() ? idx.size(-1) : 0;
+    TORCH_CHECK(K >= 1 && K <= kLmMostK, "distill: a record has 1 to 256 places");
+    const auto rows = x.sizes().slice(0, x.dim() - 1);
+    TORCH_CHECK(idx.sizes().slice(0, idx.dim() - 1) == rows &&
+                values.sizes() == idx.sizes(),
+                "distill: values and indices must be the logits' rows by k");
+    TORCH_CHECK(idx.device() == x.device() && values.device() == x.device(),
+                "distill: the record must be on the logits' device");
+    c10::DeviceGuard guard(x.device());
+    idx = idx.contiguous();
+    values = values.contiguous();
+    if (lse) lse = lm_per_row(*lse, x, torch::kFloat32, "teacher_lse");
+    if (mask) mask = lm_per_row(*mask, x, torch::kBool, "mask");
+    LmPlaces pl{};
+    lm_set_idx(&pl, idx);
+    pl.mask = (const uint8_t*)lm_ptr(mask);
+    pl.K = (int)K;
+    LmTeacher te{values.data_ptr(), (const float*)lm_ptr(lse),
+                 lm_type(values, "teacher_values"), (float)temperature};
+    LmKeep kp;
+    auto keep = lm_keep(x, in, pl.K, &kp);
+    LmOut o;
+    auto loss = lm_loss_out(x, rows, reduction, kp, &o);
+    ctx->save_for_backward({x, idx, keep});
+    ctx->saved_data["K"] = K;
+    ctx->saved_data["t"] = temperature;
+    ctx->saved_data["per"] = (int64_t)(reduction == LM_NONE ? LM_UP_ROW : LM_UP_ALL);
+    if (!in.R) return loss.zero_();
+    LmWork w;
+    auto ws = lm_work(x, in, lse.has_value(), true, lm_blocks_of_rows(in.R), &w);
+    lm_distill(in, pl, te, w, kp, o, cur_stream());
+    return loss;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    auto dx = lm_backward(ctx, grads[0], ctx->saved_data["per"].toInt(),
+                          ctx->saved_data["K"].toInt(),
+                          ctx->saved_data["t"].toDouble());
+    return {dx, {}, {}, {}, {}, {}, {}};
+  }
+};
+
+struct LmPolicyFn : public torch::autograd::Function<LmPolicyFn> {
+  static variable_list forward(AutogradContext* ctx, torch::Tensor x,
+                               torch::Tensor actions, torch::Tensor old_lp,
+                               torch::Tensor adv,
+                               c10::optional<torch::Tensor> ref_lp,
+                               c10::optional<torch::Tensor> mask,
+                               double clip_low, double clip_high,
+                               double kl_coef, int64_t reduction) {
+    LmRows in = lm_rows(x, 1.0);
+    c10::DeviceGuard guard(x.device());
+    actions = lm_per_row(actions, x, torch::kLong, "actions");
+    old_lp = lm_per_row(old_lp, x, torch::kFloat32, "old_logps");
+    adv = lm_per_row(adv, x, torch::kFloat32, "advantages");
+    if (ref_lp) ref_lp = lm_per_row(*ref_lp, x, torch::kFloat32, "ref_logps");
+    if (mask) mask = lm_per_row(*mask, x, torch::kBool, "mask");
+    LmPlaces pl{};
+    lm_set_idx(&pl, actions);
+    pl.mask = (const uint8_t*)lm_ptr(mask);
+    pl.K = 1;
+    LmPolicy po{old_lp.data_ptr<float>(), adv.data_ptr<float>(),
+                (const float*)lm_ptr(ref_lp), clip_low, clip_high, kl_coef};
+    LmKeep kp;
+    auto keep = lm_keep(x, in, 0, &kp);
+    LmOut o;
+    const auto rows = x.sizes().slice(0, x.dim() - 1);
+    auto loss = lm_loss_out(x, rows, reduction, kp, &o);
+    const auto opt = loss.options();
+    auto logps = torch::empty(rows, opt), kl = torch::empty(rows, opt);
+    ctx->save_for_backward({x, actions, keep});
+    ctx->saved_data["per"] = (int64_t)(reduction == LM_NONE ? LM_UP_ROW : LM_UP_ALL);
+    ctx->mark_non_differentiable({logps, kl});
+    ctx->set_materialize_grads(false);
+    if (!in.R) return {loss.zero_(), logps, kl};
+    LmWork w;
+    auto ws = lm_work(x, in, false, false, lm_blocks_of_rows(in.R), &w);
+    lm_policy(in, pl, po, w, kp, logps.data_ptr<float>(), kl.data_ptr<float>(), o,
+              cur_stream());
+    return {loss, logps, kl};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    torch::Tensor dx;
+    if (grads[0].defined())
+      dx = lm_backward(ctx, grads[0], ctx->saved_data["per"].toInt(), 0, 1.0);
+    return {dx, {}, {}, {}, {}, {}, {}, {}, {}, {}};
+  }
+};
+
+struct LmPreferenceFn : public torch::autograd::Function<LmPreferenceFn> {
+  static variable_list forward(AutogradContext* ctx, torch::Tensor x,
+                               torch::Tensor targets, torch::Tensor ref,
+                               double beta, double smoothing,
+                               int64_t ignore_index, int64_t reduction) {
+    LmRows in = lm_rows(x, 1.0);
+    TORCH_CHECK(x.dim() == 3 && x.size(0) % 2 == 0 && (in.T || !x.size(0)),
+                "preference: logits must be [2N, T, V] with T >= 1");
+    TORCH_CHECK(ref.device() == x.device() && ref.dim() == 1 &&
+                ref.size(0) == x.size(0), "preference: ref_logps must be [2N]");
+    c10::DeviceGuard guard(x.device());
+    targets = lm_per_row(targets, x, torch::kLong, "targets");
+    if (ref.scalar_type() != torch::kDouble) ref = ref.to(torch::kFloat32);
+    ref = ref.contiguous();
+    LmPlaces pl{};
+    lm_set_idx(&pl, targets);
+    pl.K = 1;
+    pl.use_ignore = 1;
+    pl.ignore = ignore_index;
+    LmPreference pr{ref.data_ptr(), ref.scalar_type() == torch::kDouble, beta,
+                    smoothing};
+    const int64_t N = x.size(0) / 2;
+    LmKeep kp;
+    auto keep = lm_keep(x, in, 0, &kp);
+    LmOut o;
+    auto loss = lm_loss_out(x, {N}, reduction, kp, &o);
+    const auto opt = loss.options();
+    auto chosen = torch::empty({N}, opt), rejected = torch::empty({N}, opt);
+    ctx->save_for_backward({x, targets, keep});
+    ctx->saved_data["per"] = (int64_t)(reduction == LM_NONE ? LM_UP_PAIR : LM_UP_ALL);
+    ctx->mark_non_differentiable({chosen, rejected});
+    ctx->set_materialize_grads(false);
+    if (!in.R) return {loss.zero_(), chosen, rejected};
+    LmWork w;
+    auto ws = lm_work(x, in, false, false, (int)N, &w);
+    lm_preference(in, pl, pr, w, kp, chosen.data_ptr<float>(),
+                  rejected.data_ptr<float>(), o, cur_stream());
+    return {loss, chosen, rejected};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    torch::Tensor dx;
+    if (grads[0].defined())
+      dx = lm_backward(ctx, grads[0], ctx->saved_data["per"].toInt(), 0, 1.0);
+    return {dx, {}, {}, {}, {}, {}, {}};
+  }
+};
+
+torch::Tensor lm_distill_loss(torch::Tensor x, torch::Tensor values,
+                              torch::Tensor idx, c10::optional<torch::Tensor> lse,
+                              double temperature,
+                              c10::optional<torch::Tensor> mask,
+                              int64_t reduction) {
+  return LmDistillFn::apply(x, values, idx, lse, temperature, mask, reduction);
+}
+
+// {loss, logps, kl}
+std::vector<torch::Tensor> lm_policy_loss(
+    torch::Tensor x, torch::Tensor actions, torch::Tensor old_lp,
+    torch::Tensor adv, c10::optional<torch::Tensor> ref_lp,
+    c10::optional<torch::Tensor> mask, double clip_low, double clip_high,
+    double kl_coef, int64_t reduction) {
+  return LmPolicyFn::apply(x, actions, old_lp, adv, ref_lp, mask, clip_low,
+                           clip_high, kl_coef, reduction);
+}
+
+// {loss, chosen rewards [N], rejected rewards [N]}; logits are [2N, T, V]
+std::vector<torch::Tensor> lm_preference_loss(torch::Tensor x,
+                                              torch::Tensor targets,
+                                              torch::Tensor ref, double beta,
+                                              double smoothing,
+                                              int64_t ignore_index,
+                                              int64_t reduction) {
+  return LmPreferenceFn::apply(x, targets, ref, beta, smoothing, ignore_index,
+                               reduction);
 }
 
 std::vector<torch::Tensor> rmsnorm_bwd(torch::Tensor dy, torch::Tensor x,
@@ -1398,6 +1716,13 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("colsum_bf16", &colsum_bf16, "column sum of a bf16 matrix (bias grad)");
   m.def("ce_fwd", &ce_fwd, "fused bf16 cross-entropy fwd: {loss[R], lse[R]}");
   m.def("ce_bwd", &ce_bwd, "fused bf16 cross-entropy bwd: dlogits");
+  m.def("lm_topk", &lm_topk_fwd, "k largest logits of each row + logsumexp");
+  m.def("lm_distill_loss", &lm_distill_loss,
+        "divergence from records of top logits, differentiable");
+  m.def("lm_policy_loss", &lm_policy_loss,
+        "clipped policy loss with a KL term, differentiable");
+  m.def("lm_preference_loss", &lm_preference_loss,
+        "paired log-ratio loss, differentiable");
   m.def("emb_grad_bf16", &emb_grad_bf16, "graph-safe embedding backward");
   m.def("swiglu_fwd", &swiglu_fwd);
   m.def("swiglu_bwd", &swiglu_bwd);
