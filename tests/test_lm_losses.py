@@ -115,7 +115,18 @@ def test_topk_ties_and_masks(device, dtype):
     x[6, :1000] = -5.0
     x[6, :3] = 4.0
     x[7, 4992:] = 9.0  # the largest in the last, partial vector
-    check_topk(x.to(device), 12)
+    for v in (V, 700, 4090):  # a long row, and ones that are kept whole
+        check_topk(x[:, V - v:].to(device), 12)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V,k", [(600, 256), (2100, 200), (4096, 256), (4097, 256), (8200, 256),
+                                 (33000, 256), (33000, 100), (262144, 33), (300001, 256)])
+def test_topk_piece_sizes(dtype, V, k):
+    """Around the sizes at which a row is cut into other pieces."""
+    need("cuda")
+    check_topk(make_logits(1, 3, V, dtype, "cuda")[0], k)
 
 
 @pytest.mark.parametrize("device", CPU_GPU)
@@ -236,6 +247,20 @@ def test_distill_reductions_and_upstream(device, reduction, tail):
     up = torch.randn(2, 4, generator=torch.Generator().manual_seed(3)).to(device)
     check_distill(x, values, indices.int(), lse, 1.0, None, reduction,
                   up if reduction == "none" else torch.tensor(-3.5, device=device))
+
+
+@pytest.mark.parametrize("device", CPU_GPU)
+@pytest.mark.parametrize("t", [0.05, 0.3, 0.7, 1.1, 1.5, 3.0, 4.0, 7.3, 100.0])
+def test_temperatures(device, t):
+    """Any temperature, whichever way log2(e)/t rounds; a last vector that is
+    not whole and logits of -inf."""
+    need(device)
+    x = make_logits(1, 3, 1027, torch.float32, device, scale=3.0 * min(t, 2.0))
+    x[..., 1000:] = float("-inf")
+    for tail in (False, True):
+        values, indices, lse = make_record(x, 6, t, tail=tail)
+        check_distill(x, values, indices, lse, t)
+    check_topk(x, 6, t)
 
 
 @pytest.mark.parametrize("device", CPU_GPU)

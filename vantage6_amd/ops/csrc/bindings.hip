@@ -585,7 +585,8 @@ static LmRows lm_rows(const torch::Tensor& x, double temperature) {
   in.type = lm_type(x, "logits");
   const double c = 1.4426950408889634074 / temperature;
   in.c = (float)c;
-  in.c_lo = (float)(c - in.c);
+  if ((double)in.c >= c) in.c = std::nextafterf(in.c, 0.f);
+  in.c_lo = (float)(c - in.c);  // > 0
   return in;
 }
 
@@ -619,22 +620,26 @@ static torch::Tensor lm_keep(const torch::Tensor& x, const LmRows& in, int K,
   return keep;
 }
 
-// the bytes behind a forward pass's workspaces
+// the bytes behind a forward pass's workspaces; `pairs` > 0: a block per pair
 static torch::Tensor lm_work(const torch::Tensor& x, const LmRows& in, bool rest,
-                             bool record, int blocks, LmWork* w) {
+                             bool record, int pairs, LmWork* w) {
   const long long R = in.R;
   w->splits = lm_stats_splits(in);
   lm_check_grid(in, w->splits);
+  w->group = lm_group(w->splits);
+  const int blocks = pairs ? pairs : lm_finish_blocks(in.R, w->group);
   const long long part = 8 * R * w->splits;
-  const long long n_rec = record ? 32 * R : 0, n_b = 16LL * blocks;
-  auto ws = torch::empty({n_rec + n_b + part * (rest ? 2 : 1) + 16},
+  const long long n_rec = record ? 32 * R : 0, n_xt = record ? 0 : 4 * R;
+  auto ws = torch::empty({n_rec + 16LL * blocks + part * (rest ? 2 : 1) + n_xt + 4},
                          x.options().dtype(torch::kUInt8).requires_grad(false));
   char* at = (char*)ws.data_ptr();
-  w->rec = record ? (double4*)at : nullptr;
-  w->bpart = (double2*)(at + n_rec);
-  w->part = (float2*)(at + n_rec + n_b);
-  w->part_top = rest ? (float2*)(at + n_rec + n_b + part) : nullptr;
-  w->counter = (int*)(at + n_rec + n_b + part * (rest ? 2 : 1));
+  auto next = [&at](long long n) { char* p = at; at += n; return n ? p : nullptr; };
+  w->rec = (double4*)next(n_rec);
+  w->bpart = (double2*)next(16LL * blocks);
+  w->part = (float2*)next(part);
+  w->part_top = (float2*)next(rest ? part : 0);
+  w->xt = (float*)next(n_xt);
+  w->counter = (int*)next(4);
   return ws;
 }
 
@@ -737,7 +742,7 @@ struct LmDistillFn : public torch::autograd::Function<LmDistillFn> {
     ctx->saved_data["per"] = (int64_t)(reduction == LM_NONE ? LM_UP_ROW : LM_UP_ALL);
     if (!in.R) return loss.zero_();
     LmWork w;
-    auto ws = lm_work(x, in, lse.has_value(), true, lm_blocks_of_rows(in.R), &w);
+    auto ws = lm_work(x, in, lse.has_value(), true, 0, &w);
     lm_distill(in, pl, te, w, kp, o, cur_stream());
     return loss;
   }
@@ -783,7 +788,7 @@ struct LmPolicyFn : public torch::autograd::Function<LmPolicyFn> {
     ctx->set_materialize_grads(false);
     if (!in.R) return {loss.zero_(), logps, kl};
     LmWork w;
-    auto ws = lm_work(x, in, false, false, lm_blocks_of_rows(in.R), &w);
+    auto ws = lm_work(x, in, false, false, 0, &w);
     lm_policy(in, pl, po, w, kp, logps.data_ptr<float>(), kl.data_ptr<float>(), o,
               cur_stream());
     return {loss, logps, kl};

@@ -41,8 +41,9 @@ struct LmKeep {
 
 // Workspaces of one forward pass.
 struct LmWork {
-  int splits;
-  float2 *part, *part_top;  // [splits, R]; part_top only where a record has a rest
+  int splits, group;        // blocks of a row, and lanes that join them
+  float2 *part, *part_top;  // [R, splits]; part_top only where a record has a rest
+  float* xt;                // [R], the logit of a loss's one place
   double4* rec;             // [R], distillation only
   double2* bpart;           // one per block of the finish kernel
   int* counter;
@@ -84,7 +85,8 @@ constexpr int kLmMostK = 256;
 
 int lm_stats_splits(const LmRows& in);
 int lm_grad_splits(const LmRows& in);
-int lm_blocks_of_rows(int R);
+int lm_group(int splits);
+int lm_finish_blocks(int R, int group);
 
 void lm_distill(const LmRows& in, const LmPlaces& pl, const LmTeacher& te,
                 const LmWork& w, const LmKeep& kp, const LmOut& o,

@@ -19,10 +19,12 @@
 #include "lm_loss.h"
 
 #include <cfloat>
+#include <type_traits>
 
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int Q = 4;  // 16-byte loads in flight per thread
 constexpr double kLog2e = 1.4426950408889634074;
 
 // 16 bytes at the alignment of one element: rows of an odd V start anywhere.
@@ -31,11 +33,26 @@ typedef __bf16 bf16x8_v __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8_v __attribute__((ext_vector_type(8)));
 typedef float f32x8_v __attribute__((ext_vector_type(8)));
 
+// With NT the load or store asks not to stay in the caches.
+template <bool NT>
+DEVINL u32x4 load16(const char* p) {
+  if (NT) return __builtin_nontemporal_load((const u32x4_any*)p);
+  return *(const u32x4_any*)p;
+}
+template <bool NT>
+DEVINL void store16(char* p, u32x4 v) {
+  if (NT)
+    __builtin_nontemporal_store(v, (u32x4_any*)p);
+  else
+    *(u32x4_any*)p = v;
+}
+
 template <int TY>
 struct Ty;
 template <>
 struct Ty<LM_BF16> {
   static constexpr int N = 8, size = 2, low_bits = 16;
+  static DEVINL u32x4 lowest() { return u32x4(0xff80ff80u); }  // -inf
   static DEVINL float one(const char* p) { return bf16_to_f32(*(const short*)p); }
   static DEVINL void put(char* p, float v) { *(__bf16*)p = (__bf16)v; }
   static DEVINL void open(u32x4 r, float* f) {
@@ -55,6 +72,7 @@ struct Ty<LM_BF16> {
 template <>
 struct Ty<LM_FP16> {
   static constexpr int N = 8, size = 2, low_bits = 13;
+  static DEVINL u32x4 lowest() { return u32x4(0xfc00fc00u); }
   static DEVINL float one(const char* p) { return (float)*(const _Float16*)p; }
   static DEVINL void put(char* p, float v) { *(_Float16*)p = (_Float16)v; }
   static DEVINL void open(u32x4 r, float* f) {
@@ -72,6 +90,7 @@ struct Ty<LM_FP16> {
 template <>
 struct Ty<LM_FP32> {
   static constexpr int N = 4, size = 4, low_bits = 0;
+  static DEVINL u32x4 lowest() { return u32x4(0xff800000u); }
   static DEVINL float one(const char* p) { return *(const float*)p; }
   static DEVINL void put(char* p, float v) { *(float*)p = v; }
   static DEVINL void open(u32x4 r, float* f) {
@@ -113,9 +132,40 @@ DEVINL float exp2_hw(float a) { return __builtin_amdgcn_exp2f(a); }
 
 // 2^(d log2(e)/t) with the constant in two parts: one float of it is off by up
 // to 2^-25, the same way for every logit, and that would be 1e-7 in log S, in
-// one direction for all the tokens of an answer.
+// one direction for all the tokens of an answer. The second part is positive,
+// so that a d of -inf stays one.
 DEVINL float exp_of(float d, const LmRows& in) {
   return exp2_hw(fmaf(d, in.c, d * in.c_lo));
+}
+
+// Reductions over a wave by DPP moves, a few cycles each where a shuffle
+// through LDS takes a hundred: lane ^ 1, lane ^ 2, 7 - lane of 8, 15 - lane of
+// 16, then the four rows' results. Every lane of the wave has to be there.
+template <int CTRL>
+DEVINL float moved(float v) {
+  return __int_as_float(
+      __builtin_amdgcn_mov_dpp(__float_as_int(v), CTRL, 15, 15, true));
+}
+DEVINL float lane_of(float v, int lane) {
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), lane));
+}
+DEVINL float max_of_8(float v) {
+  v = fmaxf(v, moved<0xB1>(v));
+  v = fmaxf(v, moved<0x4E>(v));
+  return fmaxf(v, moved<0x141>(v));
+}
+DEVINL float wave_max(float v) {
+  v = max_of_8(v);
+  v = fmaxf(v, moved<0x140>(v));
+  return fmaxf(fmaxf(lane_of(v, 0), lane_of(v, 16)),
+               fmaxf(lane_of(v, 32), lane_of(v, 48)));
+}
+DEVINL float wave_add(float v) {
+  v += moved<0xB1>(v);
+  v += moved<0x4E>(v);
+  v += moved<0x141>(v);
+  v += moved<0x140>(v);
+  return (lane_of(v, 0) + lane_of(v, 16)) + (lane_of(v, 32) + lane_of(v, 48));
 }
 
 // A running maximum and the sum of 2^((x-m)c) below it. m starts at the least
@@ -129,14 +179,14 @@ struct Run {
   }
 };
 DEVINL Run run_empty() { return {-FLT_MAX, 0.f}; }
+DEVINL Run wave_join(Run a, float c) {
+  const float m = wave_max(a.m);
+  return {m, wave_add(a.s * exp2_hw((a.m - m) * c))};
+}
 
 template <int THREADS>
 DEVINL Run block_join(Run a, float c, Run* red) {
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) {
-    float om = __shfl_xor(a.m, off, 64), os = __shfl_xor(a.s, off, 64);
-    a.join(om, os, c);
-  }
+  a = wave_join(a, c);
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = a;
   __syncthreads();
   a = red[0];
@@ -161,60 +211,81 @@ DEVINL double block_sum(double v, double* red) {
   return v;
 }
 
-// A record's probabilities by one block, K <= 256, in 64 bits as 1 - sum p
-// follows. rec = {sum p log p, sum p x, sum p, rest}, rest < 0 marks a row
-// without a record.
+// A record's probabilities by one wave, up to 4 of its 256 entries a lane, in
+// 64 bits as 1 - sum p follows. rec = {sum p log p, sum p x, sum p, rest},
+// rest < 0 marks a row without a record.
 DEVINL void record_of(const LmRows& in, const LmPlaces& pl, const LmTeacher& te,
                       int r, float* p_out, double4* rec) {
-  __shared__ double red[kThreads / 64];
-  __shared__ float mred[kThreads / 64];
-  const int k = threadIdx.x;
-  const long long at = (long long)r * pl.K + k;
-  const long long j = k < pl.K ? place(pl, at) : -1;
-  const float v = j >= 0 ? one_of(te.type, (const char*)te.values, at) : -INFINITY;
-  const bool some = v > -INFINITY || v != v;
-  if (__syncthreads_count(some) == 0) {
-    if (k == 0) rec[r] = make_double4(0, 0, 0, -1);
+  constexpr int E = kLmMostK / 64;
+  const int lane = threadIdx.x & 63;
+  const long long at = (long long)r * pl.K, x_at = row_start(in, r);
+  const double t = te.temperature;
+  long long j[E];
+  float v[E], m = -INFINITY;
+  bool any = false;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const int k = lane + 64 * e;
+    j[e] = k < pl.K ? place(pl, at + k) : -1;
+    v[e] = j[e] >= 0 ? one_of(te.type, (const char*)te.values, at + k) : -INFINITY;
+    any |= !(v[e] == -INFINITY);
+    m = fmaxf(m, v[e]);
+  }
+  if (!__any(any)) {
+    if (lane == 0) rec[r] = make_double4(0, 0, 0, -1);
     return;
   }
-  const double t = te.temperature;
-  double lp;
+  double lp[E], z = 0.0;
   if (te.lse) {
-    lp = (double)v / t - te.lse[r];
+#pragma unroll
+    for (int e = 0; e < E; ++e) lp[e] = (double)v[e] / t - te.lse[r];
   } else {
-    float m = v;
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
-    if ((k & 63) == 0) mred[k >> 6] = m;
-    __syncthreads();
-    m = fmaxf(fmaxf(mred[0], mred[1]), fmaxf(mred[2], mred[3]));
-    lp = ((double)v - m) / t;
-    lp -= log(block_sum(some ? exp(lp) : 0.0, red));
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      if (64 * e >= pl.K) break;
+      lp[e] = ((double)v[e] - m) / t;
+      z += v[e] == -INFINITY ? 0.0 : exp(lp[e]);
+    }
+    z = log(wave_sum(z));
   }
-  double p = some ? exp(lp) : 0.0, x = 0.0;
-  if (p != 0.0) {
-    x = j < in.V ? (double)one_of(in.type, (const char*)in.x, row_start(in, r) + j)
-                 : NAN;
-    if (j >= in.V) p = NAN;
+  double a = 0.0, b = 0.0, sum = 0.0;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    if (64 * e >= pl.K) break;
+    if (!te.lse) lp[e] -= z;
+    double p = v[e] == -INFINITY ? 0.0 : exp(lp[e]);
+    if (p != 0.0) {
+      // a place outside the row makes it a NaN
+      if (j[e] >= in.V) p = NAN;
+      const double x = j[e] < in.V
+          ? (double)one_of(in.type, (const char*)in.x, x_at + j[e]) : NAN;
+      a += p * lp[e];
+      b += p * x;
+      sum += p;
+    }
+    if (lane + 64 * e < pl.K) p_out[at + lane + 64 * e] = (float)p;
   }
-  const double a = block_sum(p != 0.0 ? p * lp : 0.0, red);
-  const double b = block_sum(p != 0.0 ? p * x : 0.0, red);
-  const double sum = block_sum(p, red);
-  if (k < pl.K) p_out[at] = (float)p;
-  if (k == 0)
+  a = wave_sum(a);
+  b = wave_sum(b);
+  sum = wave_sum(sum);
+  if (lane == 0)
     rec[r] = make_double4(a, b, sum, te.lse ? fmax(1.0 - sum, 0.0) : 0.0);
 }
 
 // ------------------------------------------------------------------- stats
-// grid R*splits, block (r, s) takes `seg` logits from s*seg on; R more blocks,
-// the first ones, make the records of a distillation. With TOP, the
-// K places of a record are kept apart: a bit per logit of the segment in LDS,
-// so that the sum outside the record is one of its own and not the difference
-// of two that nearly cancel.
-template <int TY, bool TOP>
+// Per row `splits` blocks, block s of which takes `seg` logits from s*seg on;
+// before them the blocks that make a distillation's records, a row per wave
+// (after them they would be a tail). With TOP, the K places of a record are
+// kept apart: a bit per logit of the segment in LDS, so that the sum outside
+// the record is one of its own and not the difference of two that nearly
+// cancel.
+template <int TY, bool REC, bool TOP>
 __global__ void __launch_bounds__(kThreads)
     lm_stats_kernel(LmRows in, LmPlaces pl, LmTeacher te, int splits, int seg,
-                    float2* __restrict__ part, float2* __restrict__ part_top,
+                    int keep16, float2* __restrict__ part,
+                    float2* __restrict__ part_top, float* __restrict__ xt,
                     float* __restrict__ p, double4* __restrict__ rec,
                     int* __restrict__ counter) {
   using X = Ty<TY>;
@@ -222,44 +293,64 @@ __global__ void __launch_bounds__(kThreads)
   __shared__ Run red[kThreads / 64];
   const int tid = threadIdx.x;
   if (blockIdx.x == 0 && tid == 0) *counter = 0;  // for the finish kernel
-  int at_block = blockIdx.x;
-  if (te.values) {
-    if (at_block < in.R) {
-      if (!ignored(pl, at_block)) record_of(in, pl, te, at_block, p, rec);
+  int block = blockIdx.x;
+  if (REC) {
+    constexpr int W = kThreads / 64;
+    const int records = (in.R + W - 1) / W;
+    if (block < records) {
+      const int r = block * W + (tid >> 6);
+      if (r < in.R && !ignored(pl, r)) record_of(in, pl, te, r, p, rec);
       return;
     }
-    at_block -= in.R;
+    block -= records;
   }
-  const int r = at_block / splits, sp = at_block - r * splits;
+  const int r = block / splits, sp = block - r * splits;
   if (ignored(pl, r)) return;
   const int v0 = sp * seg;
   const int n = min(seg, in.V - v0);
   const char* x = (const char*)in.x + (row_start(in, r) + v0) * X::size;
   const float c = in.c;
   const int nv = n / X::N;
+  const bool stay = (r & 15) < keep16;
+  u32x4 first[Q];
+#pragma unroll
+  for (int g = 0; g < Q; ++g) first[g] = X::lowest();
+  // two loops of loads, kept apart: the compiler would join equal loads of
+  // both branches and drop the hint
+  if (stay) {
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int g = 0; g < Q; ++g)
+      if (tid + g * kThreads < nv)
+        first[g] = load16<false>(x + (long long)(tid + g * kThreads) * 16);
+  } else {
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int g = 0; g < Q; ++g)
+      if (tid + g * kThreads < nv)
+        first[g] = load16<true>(x + (long long)(tid + g * kThreads) * 16);
+  }
+  if (xt && tid == 0) {
+    const long long j = place(pl, r);
+    if (j >= v0 && j < v0 + n)
+      xt[r] = X::one(x + (j - v0) * X::size);
+    else if (sp == 0 && (j < 0 || j >= in.V))
+      xt[r] = NAN;  // a place outside the row
+  }
   if (TOP) {
     for (int i = tid; i < (n + 31) / 32; i += kThreads) bits[i] = 0;
     __syncthreads();
-    for (int k = tid; k < pl.K; k += kThreads) {
-      long long j = place(pl, (long long)r * pl.K + k) - v0;
+    if (tid < pl.K) {
+      const long long j = place(pl, (long long)r * pl.K + tid) - v0;
       if (j >= 0 && j < n) atomicOr(&bits[j >> 5], 1u << (j & 31));
     }
     __syncthreads();
   }
   Run a = run_empty(), top = run_empty();
-  constexpr int Q = 4;  // 16-byte loads in flight per thread
-  for (int i = tid; i < nv; i += Q * kThreads) {
+  auto take = [&](const u32x4* raw, int i) {
     float f[Q * X::N];
 #pragma unroll
-    for (int g = 0; g < Q; ++g) {
-      const int ig = i + g * kThreads;
-      if (ig < nv) {
-        X::open(*(const u32x4_any*)(x + (long long)ig * 16), f + g * X::N);
-      } else {
-#pragma unroll
-        for (int e = 0; e < X::N; ++e) f[g * X::N + e] = -INFINITY;
-      }
-    }
+    for (int g = 0; g < Q; ++g) X::open(raw[g], f + g * X::N);
     if (TOP) {
 #pragma unroll
       for (int g = 0; g < Q; ++g) {
@@ -284,7 +375,32 @@ __global__ void __launch_bounds__(kThreads)
     for (int e = 0; e < Q * X::N; ++e) add[e & 3] += exp_of(f[e] - vm, in);
     a.s = a.s * exp_of(a.m - vm, in) + ((add[0] + add[1]) + (add[2] + add[3]));
     a.m = vm;
-  }
+  };
+  take(first, tid);
+  auto walk = [&](auto nt) {
+    int i = tid + Q * kThreads;
+    for (; i + (Q - 1) * kThreads < nv; i += Q * kThreads) {
+      u32x4 raw[Q];
+#pragma unroll
+      for (int g = 0; g < Q; ++g)
+        raw[g] = load16<nt.value>(x + (long long)(i + g * kThreads) * 16);
+      take(raw, i);
+    }
+    if (i < nv) {
+      u32x4 raw[Q];
+#pragma unroll
+      for (int g = 0; g < Q; ++g) {
+        raw[g] = X::lowest();
+        if (i + g * kThreads < nv)
+          raw[g] = load16<nt.value>(x + (long long)(i + g * kThreads) * 16);
+      }
+      take(raw, i);
+    }
+  };
+  if (stay)
+    walk(std::false_type());
+  else
+    walk(std::true_type());
   if (tid < n - nv * X::N) {  // what is left of a vector
     int j = nv * X::N + tid;
     float f = X::one(x + (long long)j * X::size);
@@ -299,24 +415,36 @@ __global__ void __launch_bounds__(kThreads)
     top = block_join<kThreads>(top, c, red);
   }
   if (tid == 0) {
-    long long at = (long long)sp * in.R + r;
+    const long long at = (long long)r * splits + sp;
     part[at] = make_float2(a.m, a.s);
     if (TOP) part_top[at] = make_float2(top.m, top.s);
   }
 }
 
-// the splits of a row as one, in 64 bits from here on
+// The finish kernels give a row to a group of lanes, a power of two that holds
+// the row's splits (at most a wave), and work in 64 bits from here on.
 struct Row {
   double m, s;
 };
-DEVINL Row join_splits(const float2* part, int splits, int R, int r, double c) {
+DEVINL Row join_splits(const float2* part, int splits, int group, int r,
+                       bool live, double c) {
+  const int lane = threadIdx.x & (group - 1);
   float m = -FLT_MAX;
-  for (int i = 0; i < splits; ++i) m = fmaxf(m, part[(long long)i * R + r].x);
   double s = 0.0;
-  for (int i = 0; i < splits; ++i) {
-    float2 q = part[(long long)i * R + r];
-    s += q.x == m ? (double)q.y : (double)q.y * exp2(((double)q.x - m) * c);
-  }
+  if (live)
+    for (int i = lane; i < splits; i += group) {
+      const float2 q = part[(long long)r * splits + i];
+      const float mn = fmaxf(m, q.x);
+      if (m != mn) s *= exp2(((double)m - mn) * c);
+      s += q.x == mn ? (double)q.y : (double)q.y * exp2(((double)q.x - mn) * c);
+      m = mn;
+    }
+  float all = m;
+  for (int off = 1; off < group; off <<= 1)
+    all = fmaxf(all, __shfl_xor(all, off, 64));
+  if (m != all) s *= exp2(((double)m - all) * c);
+  for (int off = 1; off < group; off <<= 1) s += __shfl_xor(s, off, 64);
+  m = all;
   return {(double)m, s};
 }
 
@@ -357,134 +485,127 @@ DEVINL void grid_mean(double loss, double count, double2* bpart, int* counter,
 
 // ------------------------------------------------------------------ distill
 __global__ void __launch_bounds__(kThreads)
-    lm_distill_kernel(LmRows in, LmPlaces pl, LmTeacher te, int splits,
-                      const float2* __restrict__ part,
-                      const float2* __restrict__ part_top,
-                      const double4* __restrict__ rec,
-                      LmStat* __restrict__ stat, float* __restrict__ coef,
-                      double2* bpart, int* counter, LmOut o) {
-  const int r = blockIdx.x * kThreads + threadIdx.x;
-  double loss = 0.0, count = 0.0;
-  if (r < in.R) {
-    LmStat st = {0.f, 0.f, 0.f, 0.f};
-    float a = 0.f;
-    const bool live = !ignored(pl, r);
-    const double4 k = live ? rec[r] : make_double4(0, 0, 0, -1);
-    if (live && !(k.w < 0.0)) {
-      const double t = te.temperature, c = kLog2e / t;
-      Row rest = join_splits(part, splits, in.R, r, c), all = rest;
-      // dL/dx_j t = mass q_j - p_j, mass = sum p + rest: 1, if the record's
-      // values and its logsumexp are of the same row
-      double tail = 0.0, mass = k.z;
-      if (te.lse) {
-        Row top = join_splits(part_top, splits, in.R, r, c);
-        all.m = fmax(rest.m, top.m);
-        double sr = rest.s * exp((rest.m - all.m) / t);
-        all.s = sr + top.s * exp((top.m - all.m) / t);
-        // no logit outside the record is above -inf: it has no rest
-        if (rest.s != 0.0) {
-          double log_rest = (rest.m - all.m) / t + log(rest.s / all.s);
-          if (k.w > 0.0) tail = k.w * (log(k.w) - log_rest);
-          mass += k.w;
-          st.w = (float)((mass * exp(log_rest) - k.w) / rest.s);
-        }
-      } else {
-        st.w = (float)(mass / all.s);
+    lm_distill_kernel(LmRows in, LmPlaces pl, LmTeacher te, LmWork w, LmKeep kp,
+                      LmOut o) {
+  const int at = blockIdx.x * blockDim.x + threadIdx.x, r = at / w.group;
+  const bool lead = (at & (w.group - 1)) == 0 && r < in.R;
+  const bool on = r < in.R && !ignored(pl, r);
+  const double4 k = on ? w.rec[r] : make_double4(0, 0, 0, -1);
+  const bool live = !(k.w < 0.0);
+  const double t = te.temperature, c = kLog2e / t;
+  const Row rest = join_splits(w.part, w.splits, w.group, r, live, c);
+  Row top = {0, 0};
+  if (te.lse) top = join_splits(w.part_top, w.splits, w.group, r, live, c);
+  LmStat st = {0.f, 0.f, 0.f, 0.f};
+  double loss = 0.0;
+  float a = 0.f;
+  if (live) {
+    Row all = rest;
+    // dL/dx_j t = mass q_j - p_j, mass = sum p + rest: 1, if the record's
+    // values and its logsumexp are of the same row
+    double tail = 0.0, mass = k.z;
+    if (te.lse) {
+      all.m = fmax(rest.m, top.m);
+      all.s = rest.s * exp((rest.m - all.m) / t) + top.s * exp((top.m - all.m) / t);
+      // no logit outside the record is above -inf: it has no rest
+      if (rest.s != 0.0) {
+        const double log_rest = (rest.m - all.m) / t + log(rest.s / all.s);
+        if (k.w > 0.0) tail = k.w * (log(k.w) - log_rest);
+        mass += k.w;
+        st.w = (float)((mass * exp(log_rest) - k.w) / rest.s);
       }
-      st.mb = (float)rest.m;
-      st.M = (float)all.m;
-      st.mass_S = (float)(mass / all.s);
-      loss = k.x - (k.y - k.z * all.m) / t + k.z * log(all.s) + tail;
-      loss *= t * t;
-      count = 1.0;
-      // d/dx of t^2 KL(x/t); a NaN, of a place outside the row too, is the
-      // whole row's
-      a = loss == loss ? (float)t : NAN;
+    } else {
+      st.w = (float)(mass / all.s);
     }
-    stat[r] = st;
-    coef[r] = a;
+    st.mb = (float)rest.m;
+    st.M = (float)all.m;
+    st.mass_S = (float)(mass / all.s);
+    loss = t * t * (k.x - (k.y - k.z * all.m) / t + k.z * log(all.s) + tail);
+    // d/dx of t^2 KL(x/t); a NaN, of a place outside the row too, is the
+    // whole row's
+    a = loss == loss ? (float)t : NAN;
+  }
+  if (lead) {
+    kp.stat[r] = st;
+    kp.coef[r] = a;
     if (o.reduction == LM_NONE) o.loss[r] = (float)loss;
   }
-  if (o.reduction != LM_NONE) grid_mean(loss, count, bpart, counter, o);
+  if (o.reduction != LM_NONE)
+    grid_mean(lead ? loss : 0.0, lead && live ? 1.0 : 0.0, w.bpart, w.counter, o);
 }
 
 // ------------------------------------------- log-probability of one token
 // lp = (x_t - M) - log S; a target outside the row gives NaN
-DEVINL double token_logp(const LmRows& in, const LmPlaces& pl, int r, int splits,
-                         const float2* part, LmStat* st) {
-  Row a = join_splits(part, splits, in.R, r, kLog2e);
-  long long j = place(pl, r);
-  double x = j >= 0 && j < in.V
-                 ? (double)one_of(in.type, (const char*)in.x, row_start(in, r) + j)
-                 : NAN;
-  float inv = (float)(1.0 / a.s);
+DEVINL double token_logp(const LmWork& w, int r, bool live, LmStat* st) {
+  const Row a = join_splits(w.part, w.splits, w.group, r, live, kLog2e);
+  *st = {0.f, 0.f, 0.f, 0.f};
+  if (!live) return 0.0;
+  const float inv = (float)(1.0 / a.s);
   *st = {(float)a.m, inv, (float)a.m, inv};
-  return (x - a.m) - log(a.s);
+  return ((double)w.xt[r] - a.m) - log(a.s);
 }
 
 __global__ void __launch_bounds__(kThreads)
-    lm_policy_kernel(LmRows in, LmPlaces pl, LmPolicy po, int splits,
-                     const float2* __restrict__ part, LmStat* __restrict__ stat,
-                     float* __restrict__ coef, float* __restrict__ logps,
-                     float* __restrict__ kls, double2* bpart, int* counter,
+    lm_policy_kernel(LmRows in, LmPlaces pl, LmPolicy po, LmWork w, LmKeep kp,
+                     float* __restrict__ logps, float* __restrict__ kls,
                      LmOut o) {
-  const int r = blockIdx.x * kThreads + threadIdx.x;
-  double loss = 0.0, count = 0.0;
-  if (r < in.R) {
-    LmStat st = {0.f, 0.f, 0.f, 0.f};
-    double by_lp = 0.0, lp = 0.0, kl = 0.0;
-    if (!ignored(pl, r)) {
-      lp = token_logp(in, pl, r, splits, part, &st);
-      const double A = po.adv[r], lo = 1.0 - po.clip_low,
-                   hi = 1.0 + po.clip_high;
-      const double ratio = exp(lp - (double)po.old_lp[r]);
-      const double held = fmin(fmax(ratio, lo), hi);
-      // the lesser of ratio*A and held*A; a NaN stays one
-      const bool moves = A > 0.0 ? !(ratio > hi) : !(ratio < lo);
-      loss = moves ? -ratio * A : -held * A;
-      by_lp = moves ? -ratio * A : 0.0;
-      if (po.ref_lp) {
-        const double d = (double)po.ref_lp[r] - lp, e = expm1(d);
-        kl = e - d;
-        loss += po.kl_coef * kl;
-        by_lp -= po.kl_coef * e;
-      }
-      count = 1.0;
+  const int at = blockIdx.x * blockDim.x + threadIdx.x, r = at / w.group;
+  const bool lead = (at & (w.group - 1)) == 0 && r < in.R;
+  const bool live = r < in.R && !ignored(pl, r);
+  double loss = 0.0, by_lp = 0.0, kl = 0.0;
+  LmStat st;
+  const double lp = token_logp(w, r, live, &st);
+  if (live) {
+    const double A = po.adv[r], lo = 1.0 - po.clip_low, hi = 1.0 + po.clip_high;
+    const double ratio = exp(lp - (double)po.old_lp[r]);
+    const double held = fmin(fmax(ratio, lo), hi);
+    // the lesser of ratio*A and held*A; a NaN stays one
+    const bool moves = A > 0.0 ? !(ratio > hi) : !(ratio < lo);
+    loss = moves ? -ratio * A : -held * A;
+    by_lp = moves ? -ratio * A : 0.0;
+    if (po.ref_lp) {
+      const double d = (double)po.ref_lp[r] - lp, e = expm1(d);
+      kl = e - d;
+      loss += po.kl_coef * kl;
+      by_lp -= po.kl_coef * e;
     }
-    stat[r] = st;
-    // the gradient is coef * (q - onehot)
-    coef[r] = (float)-by_lp;
+  }
+  if (lead) {
+    kp.stat[r] = st;
+    kp.coef[r] = (float)-by_lp;  // the gradient is coef * (q - onehot)
     logps[r] = (float)lp;
     kls[r] = (float)kl;
     if (o.reduction == LM_NONE) o.loss[r] = (float)loss;
   }
-  if (o.reduction != LM_NONE) grid_mean(loss, count, bpart, counter, o);
+  if (o.reduction != LM_NONE)
+    grid_mean(lead ? loss : 0.0, lead && live ? 1.0 : 0.0, w.bpart, w.counter, o);
 }
 
 // One block per pair: sequences n and n + N. The sums over an answer are held
 // in 64 bits, as the loss is made of the small differences between them.
 __global__ void __launch_bounds__(1024)
-    lm_preference_kernel(LmRows in, LmPlaces pl, LmPreference pr, int splits,
-                         const float2* __restrict__ part,
-                         LmStat* __restrict__ stat, float* __restrict__ coef,
-                         float* __restrict__ chosen,
-                         float* __restrict__ rejected, double2* bpart,
-                         int* counter, LmOut o) {
+    lm_preference_kernel(LmRows in, LmPlaces pl, LmPreference pr, LmWork w,
+                         LmKeep kp, float* __restrict__ chosen,
+                         float* __restrict__ rejected, LmOut o) {
   __shared__ double red[16];
   const int n = blockIdx.x, N = gridDim.x, T = in.T;
-  double sum[2];
-#pragma unroll
-  for (int side = 0; side < 2; ++side) {
-    double part_sum = 0.0;
-    const int r0 = (n + side * N) * T;
-    for (int t = threadIdx.x; t < T; t += blockDim.x) {
-      LmStat st = {0.f, 0.f, 0.f, 0.f};
-      if (!ignored(pl, r0 + t))
-        part_sum += token_logp(in, pl, r0 + t, splits, part, &st);
-      stat[r0 + t] = st;
+  const int mine = threadIdx.x / w.group, rows = blockDim.x / w.group;
+  const bool lead = (threadIdx.x & (w.group - 1)) == 0;
+  double sum[2] = {0.0, 0.0};
+  for (int t0 = 0; t0 < 2 * T; t0 += rows) {
+    const int t = t0 + mine, side = t >= T;
+    const int r = (n + side * N) * T + t - side * T;
+    const bool live = t < 2 * T && !ignored(pl, r);
+    LmStat st;
+    const double lp = token_logp(w, r, live, &st);
+    if (lead && t < 2 * T) {
+      kp.stat[r] = st;
+      sum[0] += side ? 0.0 : lp;
+      sum[1] += side ? lp : 0.0;
     }
-    sum[side] = block_sum(part_sum, red);
   }
+  sum[0] = block_sum(sum[0], red);
+  sum[1] = block_sum(sum[1], red);
   double reward[2];
 #pragma unroll
   for (int side = 0; side < 2; ++side) {
@@ -503,7 +624,7 @@ __global__ void __launch_bounds__(1024)
     const int r0 = (n + side * N) * T;
     const float a = (float)((side ? 1.0 : -1.0) * pr.beta * by_z);
     for (int t = threadIdx.x; t < T; t += blockDim.x)
-      coef[r0 + t] = ignored(pl, r0 + t) ? 0.f : a;
+      kp.coef[r0 + t] = ignored(pl, r0 + t) ? 0.f : a;
   }
   if (threadIdx.x == 0) {
     chosen[n] = (float)reward[0];
@@ -512,7 +633,7 @@ __global__ void __launch_bounds__(1024)
   }
   if (o.reduction != LM_NONE)
     grid_mean(threadIdx.x == 0 ? loss : 0.0, threadIdx.x == 0 ? 1.0 : 0.0,
-              bpart, counter, o);
+              w.bpart, w.counter, o);
 }
 
 // --------------------------------------------------------------------- grad
@@ -520,7 +641,7 @@ __global__ void __launch_bounds__(1024)
 // whose coefficient is 0 (ignored, or clipped) is not read. The rows go from
 // the last to the first, as the last ones that stats read are the likeliest
 // to be still in the cache.
-template <int TY, bool ONE>
+template <int TY, bool ONE, bool NT>
 __global__ void __launch_bounds__(kThreads)
     lm_grad_kernel(LmRows in, LmPlaces pl, LmKeep kp, LmUp up,
                    char* __restrict__ dx_all, int splits, int seg) {
@@ -544,7 +665,7 @@ __global__ void __launch_bounds__(kThreads)
   if (a == 0.f) {
     const u32x4 zero = {0, 0, 0, 0};
     for (int i = tid; i < nv; i += kThreads)
-      *(u32x4_any*)(dx + (long long)i * 16) = zero;
+      store16<NT>(dx + (long long)i * 16, zero);
     if (tid < left) X::put(dx + (long long)(nv * X::N + tid) * X::size, 0.f);
     return;
   }
@@ -552,30 +673,48 @@ __global__ void __launch_bounds__(kThreads)
   const LmStat st = kp.stat[r];
   const float c = in.c, mb = st.mb, w = a * st.w;
   const long long target = ONE ? place(pl, r) - v0 : -1;
-  constexpr int Q = 4;
-  for (int i = tid; i < nv; i += Q * kThreads) {
+  // a place of the record in this segment, and what goes there. The same
+  // index twice adds both probabilities, and both threads write one value.
+  long long at = -1;
+  float there = 0.f;
+  if (!ONE) {
+    if (tid < pl.K) {
+      at = place(pl, (long long)r * pl.K + tid) - v0;
+      s_idx[tid] = at;
+      s_p[tid] = kp.p[(long long)r * pl.K + tid];
+      if (at >= n) at = -1;
+    }
+    __syncthreads();
+    if (at >= 0) {
+      const float xt = X::one(x + at * X::size);
+      float ps = 0.f;
+      for (int k = 0; k < pl.K; ++k) ps += s_idx[k] == at ? s_p[k] : 0.f;
+      there = a * (st.mass_S * exp2_hw((xt - st.M) * c) - ps);
+    }
+  }
+  auto put = [&](u32x4 raw, int ig) {
+    float f[X::N];
+    X::open(raw, f);
+#pragma unroll
+    for (int e = 0; e < X::N; ++e) f[e] = w * exp2_hw((f[e] - mb) * c);
+    if (ONE && target >= (long long)ig * X::N &&
+        target < (long long)(ig + 1) * X::N) {
+#pragma unroll
+      for (int e = 0; e < X::N; ++e)
+        if (target == (long long)ig * X::N + e) f[e] -= a;
+    }
+    store16<NT>(dx + (long long)ig * 16, X::close(f));
+  };
+  int i = tid;
+  for (; i + (Q - 1) * kThreads < nv; i += Q * kThreads) {
     u32x4 raw[Q];
 #pragma unroll
     for (int g = 0; g < Q; ++g)
-      if (i + g * kThreads < nv)
-        raw[g] = *(const u32x4_any*)(x + (long long)(i + g * kThreads) * 16);
+      raw[g] = load16<true>(x + (long long)(i + g * kThreads) * 16);
 #pragma unroll
-    for (int g = 0; g < Q; ++g) {
-      const int ig = i + g * kThreads;
-      if (ig >= nv) break;
-      float f[X::N];
-      X::open(raw[g], f);
-#pragma unroll
-      for (int e = 0; e < X::N; ++e) f[e] = w * exp2_hw((f[e] - mb) * c);
-      if (ONE && target >= (long long)ig * X::N &&
-          target < (long long)(ig + 1) * X::N) {
-#pragma unroll
-        for (int e = 0; e < X::N; ++e)
-          if (target == (long long)ig * X::N + e) f[e] -= a;
-      }
-      *(u32x4_any*)(dx + (long long)ig * 16) = X::close(f);
-    }
+    for (int g = 0; g < Q; ++g) put(raw[g], i + g * kThreads);
   }
+  for (; i < nv; i += kThreads) put(load16<true>(x + (long long)i * 16), i);
   if (tid < left) {
     const int j = nv * X::N + tid;
     float f = w * exp2_hw((X::one(x + (long long)j * X::size) - mb) * c);
@@ -583,180 +722,299 @@ __global__ void __launch_bounds__(kThreads)
     X::put(dx + (long long)j * X::size, f);
   }
   if (!ONE) {
-    // the record's places: the same index twice adds both probabilities, and
-    // both threads write the same value
-    if (tid < pl.K) {
-      s_idx[tid] = place(pl, (long long)r * pl.K + tid) - v0;
-      s_p[tid] = kp.p[(long long)r * pl.K + tid];
-    }
-    __syncthreads();
-    if (tid < pl.K) {
-      const long long j = s_idx[tid];
-      if (j >= 0 && j < n) {
-        float ps = 0.f;
-        for (int k = 0; k < pl.K; ++k) ps += s_idx[k] == j ? s_p[k] : 0.f;
-        const float q =
-            st.mass_S * exp2_hw((X::one(x + j * X::size) - st.M) * c);
-        X::put(dx + j * X::size, a * (q - ps));
-      }
-    }
+    __syncthreads();  // the row is written, now its places
+    if (at >= 0) X::put(dx + at * X::size, there);
   }
 }
 
 // --------------------------------------------------------------------- topk
-// One block per row. Thread c owns the vectors c, c + THREADS, ...; the k-th
-// largest of the threads' maxima is a bound below the k-th largest logit, as
-// k logits reach it. Only the threads' shares whose maximum reaches the bound
-// are read again (about k of them, so some k/THREADS of the row, from the
-// cache), and the few logits that reach it are ranked by counting. Rows that
-// break this (a long run of equal logits, fewer finite ones than k) find the
-// k-th key by bisection over the whole row.
-DEVINL unsigned order_key(float f) {
-  if (f != f) return 0xffffffffu;  // above all, as in torch
-  unsigned u = __float_as_uint(f + 0.f);  // -0 and 0 are equal
+// One block per row. The row falls into pieces, and the k-th largest of their
+// maxima is a bound below the k-th largest logit, as k logits reach it. Only
+// the pieces whose maximum reaches the bound are read again, and the few logits
+// that reach it are ranked by counting. A piece is one logit (PIECE = 0) where
+// all fit into LDS, else a vector of 16 bytes, or a line of eight vectors where
+// those are many: of 128256 logits in 16 bits 2004 lines, of which some k are
+// read again. Rows that break this (a long run of equal logits, a NaN or +inf)
+// find the k-th key by bisection over the whole row.
+enum { kLogits = 0, kVectors = 1, kLines = 8 };
+
+DEVINL unsigned order_of(float f) {  // not for a NaN
+  const unsigned u = __float_as_uint(f + 0.f);  // -0 and 0 are equal
   return u ^ ((int)u < 0 ? 0xffffffffu : 0x80000000u);
 }
+DEVINL unsigned order_key(float f) {
+  return f != f ? 0xffffffffu : order_of(f);  // above all, as in torch
+}
 
-constexpr int kCand = 1024;
+constexpr int kCand = 2048;    // logits that reach the bound
+constexpr int kPieces = 4096;  // maxima kept; piece i of a longer row is in i % kPieces
 
-template <int TY, int THREADS>
+// a logit that ranks, its place, and whether its zero was a negative one
+DEVINL unsigned long long candidate(float f, int j) {
+  return (unsigned long long)order_key(f) << 32 | (unsigned)(0x3fffffff - j) << 1 |
+         (__float_as_uint(f) == 0x80000000u);
+}
+DEVINL int place_of(unsigned long long cand) {
+  return 0x3fffffff - (int)((unsigned)cand >> 1);
+}
+DEVINL float logit_of(unsigned long long cand) {
+  const unsigned u = (unsigned)(cand >> 32);
+  if (cand & 1) return -0.f;
+  return __uint_as_float(u == 0xffffffffu ? 0x7fc00000u
+                         : u & 0x80000000u ? u ^ 0x80000000u : ~u);
+}
+
+template <int TY, int THREADS, int PIECE, bool NT>
 __global__ void __launch_bounds__(THREADS)
-    lm_topk_kernel(LmRows in, float temperature, int k, char* __restrict__ values,
+    lm_topk_kernel(LmRows in, float temperature, int k,
+                   char* __restrict__ values,
                    long long* __restrict__ indices, float* __restrict__ lse) {
   using X = Ty<TY>;
   __shared__ Run red[THREADS / 64];
-  __shared__ unsigned keys[THREADS];
+  __shared__ __align__(16) float maxima[kPieces];
   __shared__ unsigned long long cand[kCand];
-  __shared__ int share[THREADS];
-  __shared__ int n_share, n_cand, total;
-  __shared__ unsigned s_bound;
+  __shared__ unsigned short share[kPieces];
+  __shared__ int n_share, n_cand, total, odd;
+  __shared__ float s_bound;
+  __shared__ Run s_run;
   const int tid = threadIdx.x, r = blockIdx.x;
   const char* x = (const char*)in.x + row_start(in, r) * X::size;
   const float c = in.c;
   const int V = in.V, nv = V / X::N, left = V - nv * X::N;
-  if (tid == 0) n_share = n_cand = 0;
+  if (tid == 0) n_share = n_cand = odd = 0;
+  for (int i = tid; i < kPieces; i += THREADS) maxima[i] = -INFINITY;
+  __syncthreads();
 
   Run a = run_empty();
-  float mx = -INFINITY;
-  constexpr int Q = 4;
-  for (int i = tid; i < nv; i += Q * THREADS) {
-    float f[Q * X::N];
+  constexpr int SHIFT = PIECE == kLines ? 3 : 0;  // vectors of a piece
+  const int pieces = PIECE == kLogits ? V : (nv + (1 << SHIFT) - 1) >> SHIFT;
+  const bool folded = pieces > kPieces;
+  auto take = [&](const u32x4* raw, int i) {
+    float f[Q * X::N], vm = a.m;
 #pragma unroll
     for (int g = 0; g < Q; ++g) {
-      const int ig = i + g * THREADS;
-      if (ig < nv) {
-        u32x4 raw = *(const u32x4_any*)(x + (long long)ig * 16);
-        X::open(raw, f + g * X::N);
-      } else {
+      X::open(raw[g], f + g * X::N);
+      float m = f[g * X::N];
 #pragma unroll
-        for (int e = 0; e < X::N; ++e) f[g * X::N + e] = -INFINITY;
+      for (int e = 1; e < X::N; ++e) m = fmaxf(m, f[g * X::N + e]);
+      vm = fmaxf(vm, m);
+      // one lane writes a place of `maxima`, in all rounds of a long row
+      static_assert(kPieces % THREADS == 0, "a place has one writer");
+      const int ig = i + g * THREADS;
+      if (PIECE == kLogits) {
+        if (ig < nv) {
+#pragma unroll
+          for (int e = 0; e < X::N; ++e) maxima[ig * X::N + e] = f[g * X::N + e];
+        }
+        continue;
+      }
+      if (SHIFT) m = max_of_8(m);
+      if ((!SHIFT || (tid & 7) == 0) && ig < nv) {
+        float* at = &maxima[(ig >> SHIFT) & (kPieces - 1)];
+        *at = folded ? fmaxf(*at, m) : m;
       }
     }
-#pragma unroll
-    for (int e = 0; e < Q * X::N; ++e) mx = fmaxf(mx, f[e]);
-    const float vm = fmaxf(a.m, mx);
+    // log S needs no second part of the constant here: 1e-7 is less than half
+    // a step of its float
     float add[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int e = 0; e < Q * X::N; ++e) add[e & 3] += exp_of(f[e] - vm, in);
-    a.s = a.s * exp_of(a.m - vm, in) + ((add[0] + add[1]) + (add[2] + add[3]));
+    for (int e = 0; e < Q * X::N; ++e) add[e & 3] += exp2_hw((f[e] - vm) * c);
+    a.s = a.s * exp2_hw((a.m - vm) * c) + ((add[0] + add[1]) + (add[2] + add[3]));
     a.m = vm;
-  }
-  // a NaN hides from fmaxf but not from the sum; +inf, which also makes the
-  // sum one, is a bound below either
-  unsigned key = tid < nv ? order_key(a.s != a.s ? INFINITY : mx) : 0u;
-  keys[tid] = key;
-  if (tid < left) a.join(X::one(x + (long long)(nv * X::N + tid) * X::size), 1.f, c);
-  a = block_join<THREADS>(a, c, red);
-  if (tid == 0)  // a row of -inf: log 0
-    lse[r] = (float)((double)a.m / temperature + log((double)a.s));
-  if (tid < 64) {
-    unsigned mine[THREADS / 64], t = 0;
+  };
+  // whole waves go the same way: max_of_8 needs all its lanes
+  int i = tid;
+  for (; (i | 63) + (Q - 1) * THREADS < nv; i += Q * THREADS) {
+    u32x4 raw[Q];
 #pragma unroll
-    for (int i = 0; i < THREADS / 64; ++i) mine[i] = keys[i * 64 + tid];
-    for (int bit = 31; bit >= X::low_bits; --bit) {
-      const unsigned trial = t | (1u << bit);
+    for (int g = 0; g < Q; ++g)
+      raw[g] = load16<NT>(x + (long long)(i + g * THREADS) * 16);
+    take(raw, i);
+  }
+  if ((i & ~63) < nv) {
+    u32x4 raw[Q];
+#pragma unroll
+    for (int g = 0; g < Q; ++g) {
+      raw[g] = X::lowest();
+      if (i + g * THREADS < nv)
+        raw[g] = load16<NT>(x + (long long)(i + g * THREADS) * 16);
+    }
+    take(raw, i);
+  }
+  if (tid < left) {
+    const float f = X::one(x + (long long)(nv * X::N + tid) * X::size);
+    if (PIECE == kLogits) maxima[nv * X::N + tid] = f;
+    a.join(f, 1.f, c);
+  }
+  a = wave_join(a, c);
+  if ((tid & 63) == 0) red[tid >> 6] = a;
+  __syncthreads();
+  if (tid < 64) {
+    // The bound: any t that not many more than k maxima reach will do, and a few
+    // maxima may go as one, which is a bound as well: 512 groups of them, or
+    // 1024 where k is more than a quarter of that, as a bound that most groups
+    // reach is a low one. Bit by bit from the first in which the finite ones
+    // differ.
+    constexpr int E = 16;
+    const int groups = k <= 128 ? 512 : 1024;
+    const int rounds = (min(pieces, kPieces) + groups - 1) / groups;
+    unsigned mine[E];
+    float m[E], least = INFINITY, most = -INFINITY;
+#pragma unroll
+    for (int e = 0; e < E; ++e) m[e] = -INFINITY;
+    for (int i = 0; i < rounds; ++i)
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (e * 64 < groups) m[e] = fmaxf(m[e], maxima[i * groups + e * 64 + tid]);
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      mine[e] = order_of(m[e]);
+      least = fminf(least, m[e] > -INFINITY ? m[e] : INFINITY);
+      most = fmaxf(most, m[e]);
+    }
+    const unsigned low = order_of(-wave_max(-least)), high = order_of(wave_max(most));
+    auto reach = [&](unsigned trial) {
       int cnt = 0;
 #pragma unroll
-      for (int i = 0; i < THREADS / 64; ++i)
-        cnt += __popcll(__ballot(mine[i] >= trial));
-      if (cnt >= k) {
-        t = trial;
-        if (cnt <= k + (k >> 2)) break;  // near enough
+      for (int e = 0; e < E; ++e) {
+        if (e * 64 >= groups) break;
+        cnt += __popcll(__builtin_amdgcn_ballot_w64(mine[e] >= trial));
+      }
+      return cnt;
+    };
+    unsigned t = 0;
+    if (low <= high && reach(low) >= k) {  // else there are too few
+      int bit = low == high ? -1 : 31 - __clz((int)(low ^ high));
+      t = bit < 0 ? low : low & ~((2u << bit) - 1u);
+      for (; bit >= X::low_bits; --bit) {
+        const unsigned trial = t | (1u << bit);
+        const int cnt = reach(trial);
+        if (cnt >= k) {
+          t = trial;
+          if (cnt <= k + (k >> 3) + 4) break;
+        }
       }
     }
-    if (tid == 0) s_bound = t;
+    // keys up to that of -inf stand for no float
+    if (tid == 0)
+      s_bound = t <= order_of(-INFINITY) ? -INFINITY
+                                          : logit_of((unsigned long long)t << 32);
+  } else if (tid < 128) {
+    // meanwhile another wave joins the sums
+    constexpr int W = THREADS / 64;
+    a = (tid & 63) < W ? red[tid & 63] : run_empty();
+    a = wave_join(a, c);
+    if (tid == 64) {
+      s_run = a;
+      odd = a.s != a.s;  // a NaN hides from fmaxf, but not from the sum
+    }
   }
   __syncthreads();
-  const unsigned bound = s_bound;
+  const float bound = s_bound;
   auto offer = [&](float f, int j) {
-    const unsigned o = order_key(f);
-    if (o >= bound) {
-      const int at = atomicAdd(&n_cand, 1);
-      if (at < kCand)
-        cand[at] = (unsigned long long)o << 32 | (0xffffffffu - (unsigned)j);
-    }
+    const int at = atomicAdd(&n_cand, 1);
+    if (at < kCand) cand[at] = candidate(f, j);
   };
-  if (key >= bound && tid < nv) share[atomicAdd(&n_share, 1)] = tid;
-  if (tid < left) offer(X::one(x + (long long)(nv * X::N + tid) * X::size), nv * X::N + tid);
-  __syncthreads();
-  const int deep = (nv + THREADS - 1) / THREADS, work = n_share * deep;
-  for (int i = tid; i < work; i += THREADS) {
-    const int q = i / deep;
-    const int ig = share[q] + (i - q * deep) * THREADS;
-    if (ig < nv) {
-      float f[X::N];
-      X::open(*(const u32x4_any*)(x + (long long)ig * 16), f);
-#pragma unroll
-      for (int e = 0; e < X::N; ++e) offer(f[e], ig * X::N + e);
+  for (int i = tid; i < min(pieces, kPieces); i += THREADS)
+    if (maxima[i] >= bound) {
+      if (PIECE == kLogits)
+        offer(maxima[i], i);
+      else
+        share[atomicAdd(&n_share, 1)] = (unsigned short)i;
     }
+  if (PIECE != kLogits && tid < left) {
+    const int j = nv * X::N + tid;
+    const float f = X::one(x + (long long)j * X::size);
+    if (f >= bound) offer(f, j);
   }
+  __syncthreads();
+  if (PIECE != kLogits && !odd)
+    for (int from = 0; from < pieces; from += kPieces) {
+      const int work = n_share << SHIFT;
+      for (int i = tid; i < work; i += THREADS) {
+        const int ig = ((from + share[i >> SHIFT]) << SHIFT) + (i & ((1 << SHIFT) - 1));
+        if (ig >= nv) continue;
+        float f[X::N];
+        X::open(*(const u32x4_any*)(x + (long long)ig * 16), f);
+        int hits = 0;
+#pragma unroll
+        for (int e = 0; e < X::N; ++e) hits += f[e] >= bound;
+        if (!hits) continue;
+        int at = atomicAdd(&n_cand, hits);
+#pragma unroll
+        for (int e = 0; e < X::N; ++e)
+          if (f[e] >= bound) {
+            if (at < kCand) cand[at] = candidate(f[e], ig * X::N + e);
+            ++at;
+          }
+      }
+    }
   __syncthreads();
   int nc = n_cand;
-  if (nc > kCand || nc < k) {
-    // the k-th largest (key, place) by bisection, all keys being different
+  if (odd || nc > kCand || nc < k) {
+    // The k-th largest (key, place) by bisection, all of them being different:
+    // the bits of the key, then those of a place below V.
+    auto each = [&](auto&& use) {
+      for (int i = tid; i < nv; i += THREADS) {
+        float f[X::N];
+        X::open(load16<false>(x + (long long)i * 16), f);
+#pragma unroll
+        for (int e = 0; e < X::N; ++e) use(candidate(f[e], i * X::N + e));
+      }
+      if (tid < left) {
+        const int j = nv * X::N + tid;
+        use(candidate(X::one(x + (long long)j * X::size), j));
+      }
+    };
     unsigned long long t = 0;
-    for (int bit = 63; bit >= 0; --bit) {
+    auto settle = [&](int bit) {
       const unsigned long long trial = t | 1ull << bit;
       __syncthreads();
       if (tid == 0) total = 0;
       __syncthreads();
       int mine = 0;
-      for (int j = tid; j < V; j += THREADS) {
-        const unsigned long long o =
-            (unsigned long long)order_key(X::one(x + (long long)j * X::size)) << 32 |
-            (0xffffffffu - (unsigned)j);
-        mine += o >= trial;
-      }
+      each([&](unsigned long long o) { mine += o >= trial; });
 #pragma unroll
       for (int off = 32; off > 0; off >>= 1) mine += __shfl_xor(mine, off, 64);
       if ((tid & 63) == 0) atomicAdd(&total, mine);
       __syncthreads();
       if (total >= k) t = trial;
-    }
+    };
+    for (int bit = 63; bit >= 32 + X::low_bits; --bit) settle(bit);
+    // the bits that a shorter type lacks are ones below zero, and in a NaN
+    constexpr unsigned low = (1u << X::low_bits) - 1u;
+    unsigned top = (unsigned)(t >> 32);
+    if (!(top & 0x80000000u) || (top | low) == 0xffffffffu) top |= low;
+    // as are the upper bits of every place's complement
+    const int nb = 32 - __clz((V - 1) | 1);
+    t = (unsigned long long)top << 32 | (0x3fffffffu >> nb << nb) << 1;
+    for (int bit = nb; bit > 0; --bit) settle(bit);
     __syncthreads();
     if (tid == 0) n_cand = 0;
     __syncthreads();
-    for (int j = tid; j < V; j += THREADS) {
-      const unsigned long long o =
-          (unsigned long long)order_key(X::one(x + (long long)j * X::size)) << 32 |
-          (0xffffffffu - (unsigned)j);
+    each([&](unsigned long long o) {
       if (o >= t) cand[atomicAdd(&n_cand, 1)] = o;
-    }
+    });
     __syncthreads();
     nc = n_cand;
   }
-  for (int i = tid; i < nc; i += THREADS) {
-    const unsigned long long mine = cand[i];
+  // the last wave has the fewest candidates; a row of -inf: log 0
+  if (tid == THREADS - 1)
+    lse[r] = (float)((double)s_run.m / temperature + log((double)s_run.s));
+  // rank by counting, 8 lanes to a candidate
+  for (int i0 = 0; i0 < nc; i0 += THREADS / 8) {
+    const int i = i0 + (tid >> 3);
+    const unsigned long long mine = i < nc ? cand[i] : ~0ull;
     int rank = 0;
-    for (int q = 0; q < nc; ++q) rank += cand[q] > mine;
-    if (rank < k) {
-      const unsigned j = 0xffffffffu - (unsigned)mine;
+#pragma unroll 4
+    for (int q = tid & 7; q < nc; q += 8) rank += cand[q] > mine;
+    rank += __builtin_amdgcn_mov_dpp(rank, 0xB1, 15, 15, true);
+    rank += __builtin_amdgcn_mov_dpp(rank, 0x4E, 15, 15, true);
+    rank += __builtin_amdgcn_mov_dpp(rank, 0x141, 15, 15, true);
+    if ((tid & 7) == 0 && i < nc && rank < k) {
       const long long at = (long long)r * k + rank;
-      indices[at] = j;
-      if (X::size == 2)
-        ((short*)values)[at] = ((const short*)x)[j];
-      else
-        ((int*)values)[at] = ((const int*)x)[j];
+      indices[at] = place_of(mine);
+      X::put(values + at * X::size, logit_of(mine));
     }
   }
 }
@@ -775,8 +1033,30 @@ int splits_for(const LmRows& in, int blocks, int seg_most, int* seg) {
   return div_up(in.V, *seg);
 }
 
+constexpr long long kMB = 1 << 20;
+long long bytes_of(const LmRows& in) {
+  return (long long)in.R * in.V * (in.type == LM_FP32 ? 4 : 2);
+}
+
 constexpr int kStatBlocks = 1024, kStatSeg = 131072;
 constexpr int kGradBlocks = 2048, kGradSeg = 32768;
+// Blocks of 512 threads cost the same at 1024 rows of 128256 (56 us), those of
+// 256 more (64).
+constexpr int kTopkThreads = 1024;
+
+// What the pass over a row leaves in the 256 MB cache behind the L2, the pass
+// of the gradient need not fetch again. At 525 MB of logits a cache that every
+// line goes through keeps little of them: stats + grad take 94 + 178 us, 82 +
+// 196 where all of stats' loads are told not to stay, and 88 + 162 where those
+// of 9 rows of 16 may. At 200 MB all may stay (36 + 60 us, else 37 + 70).
+constexpr long long kKeepBytes = 300 * kMB;
+// A gradient of this size is gone from the caches before anyone reads it, and
+// written past them it leaves them the logits (81 MB: 28 against 32 us, 203
+// MB: 59 against 68); a smaller one stays for the product that follows.
+constexpr long long kStreamGrad = 64 * kMB;
+// topk reads a row once and its best lines again: streamed at 263 MB 56 against
+// 60 us, at 78 MB 22 against 20.
+constexpr long long kStreamTopk = 128 * kMB;
 
 template <int TY>
 void grad_of(const LmRows& in, const LmPlaces& pl, const LmKeep& kp,
@@ -784,12 +1064,10 @@ void grad_of(const LmRows& in, const LmPlaces& pl, const LmKeep& kp,
   int seg;
   const int splits = splits_for(in, kGradBlocks, kGradSeg, &seg);
   const dim3 grid((unsigned)in.R * splits);
-  if (!kp.p)
-    lm_grad_kernel<TY, true><<<grid, kThreads, 0, s>>>(in, pl, kp, up,
-                                                       (char*)dx, splits, seg);
-  else
-    lm_grad_kernel<TY, false><<<grid, kThreads, 0, s>>>(in, pl, kp, up,
-                                                        (char*)dx, splits, seg);
+  const bool nt = bytes_of(in) > kStreamGrad;
+  auto kernel = kp.p ? (nt ? lm_grad_kernel<TY, false, true> : lm_grad_kernel<TY, false, false>)
+                     : (nt ? lm_grad_kernel<TY, true, true> : lm_grad_kernel<TY, true, false>);
+  kernel<<<grid, kThreads, 0, s>>>(in, pl, kp, up, (char*)dx, splits, seg);
 }
 
 template <int TY>
@@ -797,20 +1075,31 @@ void stats_of(const LmRows& in, const LmPlaces& pl, const LmTeacher& te,
               const LmWork& w, const LmKeep& kp, hipStream_t s) {
   int seg;
   const int splits = splits_for(in, kStatBlocks, kStatSeg, &seg);
-  const dim3 grid((unsigned)in.R * (splits + (te.values ? 1 : 0)));
-  if (w.part_top)
-    lm_stats_kernel<TY, true><<<grid, kThreads, (seg + 31) / 32 * 4, s>>>(
-        in, pl, te, splits, seg, w.part, w.part_top, kp.p, w.rec, w.counter);
-  else
-    lm_stats_kernel<TY, false><<<grid, kThreads, 0, s>>>(
-        in, pl, te, splits, seg, w.part, w.part_top, kp.p, w.rec, w.counter);
+  const dim3 grid((unsigned)in.R * splits +
+                  (te.values ? div_up(in.R, kThreads / 64) : 0));
+  const int keep16 = (int)std::min(16LL, 16 * kKeepBytes / bytes_of(in));
+  const bool top = w.part_top != nullptr;
+  auto kernel = top         ? lm_stats_kernel<TY, true, true>
+                : te.values ? lm_stats_kernel<TY, true, false>
+                            : lm_stats_kernel<TY, false, false>;
+  kernel<<<grid, kThreads, top ? (seg + 31) / 32 * 4 : 0, s>>>(
+      in, pl, te, splits, seg, keep16, w.part, w.part_top, w.xt, kp.p, w.rec,
+      w.counter);
 }
 
 template <int TY>
 void topk_of(const LmRows& in, float temperature, int k, void* values,
              long long* indices, float* lse, hipStream_t s) {
-  lm_topk_kernel<TY, 1024><<<dim3(in.R), 1024, 0, s>>>(
-      in, temperature, k, (char*)values, indices, lse);
+  constexpr int T = kTopkThreads;
+  const bool nt = bytes_of(in) > kStreamTopk;
+  const int nv = in.V / Ty<TY>::N;
+  // lines where there are four of them and more to each of the k
+  const int piece = in.V <= kPieces ? kLogits : nv >= 32 * k ? kLines : kVectors;
+  auto kernel =
+      piece == kLogits  ? (nt ? lm_topk_kernel<TY, T, kLogits, true> : lm_topk_kernel<TY, T, kLogits, false>)
+      : piece == kLines ? (nt ? lm_topk_kernel<TY, T, kLines, true> : lm_topk_kernel<TY, T, kLines, false>)
+                        : (nt ? lm_topk_kernel<TY, T, kVectors, true> : lm_topk_kernel<TY, T, kVectors, false>);
+  kernel<<<dim3(in.R), T, 0, s>>>(in, temperature, k, (char*)values, indices, lse);
 }
 
 #define LM_BY_TYPE(type, call)            \
@@ -844,24 +1133,39 @@ int lm_grad_splits(const LmRows& in) {
   return splits_for(in, kGradBlocks, kGradSeg, &seg);
 }
 
-int lm_blocks_of_rows(int R) { return div_up(R, kThreads); }
+int lm_group(int splits) {
+  int g = 1;
+  while (g < splits && g < 64) g <<= 1;
+  return g;
+}
+
+// The finish kernels are a chain of latencies: one block where it holds all the
+// rows, so that no block waits for another, else blocks of a wave while they
+// are a few hundred.
+static int finish_threads(int R, int group) {
+  const long long lanes = (long long)R * group;
+  return lanes <= kThreads ? (int)(lanes + 63) / 64 * 64 : lanes <= 16384 ? 64 : kThreads;
+}
+
+int lm_finish_blocks(int R, int group) {
+  return div_up((long long)R * group, finish_threads(R, group));
+}
 
 void lm_distill(const LmRows& in, const LmPlaces& pl, const LmTeacher& te,
                 const LmWork& w, const LmKeep& kp, const LmOut& o,
                 hipStream_t s) {
   stats(in, pl, te, w, kp, s);
-  lm_distill_kernel<<<dim3(lm_blocks_of_rows(in.R)), kThreads, 0, s>>>(
-      in, pl, te, w.splits, w.part, w.part_top, w.rec, kp.stat, kp.coef,
-      w.bpart, w.counter, o);
+  lm_distill_kernel<<<dim3(lm_finish_blocks(in.R, w.group)),
+                      finish_threads(in.R, w.group), 0, s>>>(in, pl, te, w, kp, o);
 }
 
 void lm_policy(const LmRows& in, const LmPlaces& pl, const LmPolicy& po,
                const LmWork& w, const LmKeep& kp, float* logps, float* kl,
                const LmOut& o, hipStream_t s) {
   stats(in, pl, LmTeacher{}, w, kp, s);
-  lm_policy_kernel<<<dim3(lm_blocks_of_rows(in.R)), kThreads, 0, s>>>(
-      in, pl, po, w.splits, w.part, kp.stat, kp.coef, logps, kl, w.bpart,
-      w.counter, o);
+  lm_policy_kernel<<<dim3(lm_finish_blocks(in.R, w.group)),
+                     finish_threads(in.R, w.group), 0, s>>>(in, pl, po, w, kp,
+                                                            logps, kl, o);
 }
 
 void lm_preference(const LmRows& in, const LmPlaces& pl, const LmPreference& pr,
@@ -869,10 +1173,10 @@ void lm_preference(const LmRows& in, const LmPlaces& pl, const LmPreference& pr,
                    float* rejected, const LmOut& o, hipStream_t s) {
   stats(in, pl, LmTeacher{}, w, kp, s);
   const int pairs = in.R / in.T / 2;
-  const int threads = std::min(1024, std::max(64, div_up(in.T, 64) * 64));
-  lm_preference_kernel<<<dim3(pairs), threads, 0, s>>>(
-      in, pl, pr, w.splits, w.part, kp.stat, kp.coef, chosen, rejected, w.bpart,
-      w.counter, o);
+  const long long lanes = 2LL * in.T * w.group;
+  const int threads = (int)std::min(1024LL, (lanes + 63) / 64 * 64);
+  lm_preference_kernel<<<dim3(pairs), threads, 0, s>>>(in, pl, pr, w, kp, chosen,
+                                                       rejected, o);
 }
 
 void lm_grad(const LmRows& in, const LmPlaces& pl, const LmKeep& kp,
