@@ -602,6 +602,7 @@ static torch::Tensor lm_per_row(const torch::Tensor& t, const torch::Tensor& x,
   TORCH_CHECK(t.device() == x.device(), what, " must be on the logits' device");
   TORCH_CHECK(t.sizes() == x.sizes().slice(0, x.dim() - 1), what,
               " must have the shape of the logits' rows");
+  if (t.scalar_type() == type && t.is_contiguous()) return t;
   return t.to(type).contiguous();
 }
 
@@ -609,38 +610,38 @@ static const void* lm_ptr(const c10::optional<torch::Tensor>& t) {
   return t.has_value() ? t->data_ptr() : nullptr;
 }
 
-// keep: {stat [R] of 4, coef [R], inv, p [R, K]} floats
-static torch::Tensor lm_keep(const torch::Tensor& x, const LmRows& in, int K,
-                             LmKeep* kp) {
-  const long long R = in.R;
-  auto keep = torch::empty({R * (5 + K) + 1},
-                           x.options().dtype(torch::kFloat32).requires_grad(false));
+// What the forward pass keeps, and behind it its workspaces, in one allocation:
+// stat [R] of 4 floats, coef [R], inv, p [R, K].
+static long long lm_kept(long long R, long long K) { return R * (5 + K) + 1; }
+
+static LmKeep lm_keep_of(const torch::Tensor& keep, long long R, long long K) {
   float* f = keep.data_ptr<float>();
-  *kp = {(LmStat*)f, f + 4 * R, f + 5 * R, K ? f + 5 * R + 1 : nullptr};
-  return keep;
+  return {(LmStat*)f, f + 4 * R, f + 5 * R, K ? f + 5 * R + 1 : nullptr};
 }
 
-// the bytes behind a forward pass's workspaces; `pairs` > 0: a block per pair
-static torch::Tensor lm_work(const torch::Tensor& x, const LmRows& in, bool rest,
-                             bool record, int pairs, LmWork* w) {
+// `pairs` > 0: the finish kernel has a block per pair
+static torch::Tensor lm_keep(const torch::Tensor& x, const LmRows& in, int K,
+                             bool rest, int pairs, LmKeep* kp, LmWork* w) {
   const long long R = in.R;
-  w->splits = lm_stats_splits(in);
+  w->splits = R ? lm_stats_splits(in) : 1;
   lm_check_grid(in, w->splits);
   w->group = lm_group(w->splits);
-  const int blocks = pairs ? pairs : lm_finish_blocks(in.R, w->group);
-  const long long part = 8 * R * w->splits;
-  const long long n_rec = record ? 32 * R : 0, n_xt = record ? 0 : 4 * R;
-  auto ws = torch::empty({n_rec + 16LL * blocks + part * (rest ? 2 : 1) + n_xt + 4},
-                         x.options().dtype(torch::kUInt8).requires_grad(false));
-  char* at = (char*)ws.data_ptr();
-  auto next = [&at](long long n) { char* p = at; at += n; return n ? p : nullptr; };
+  const long long part = 2 * R * w->splits;  // all in floats
+  const long long n_rec = K ? 8 * R : 0, n_xt = K ? 0 : R;
+  const long long n_b = 4LL * (pairs ? pairs : lm_finish_blocks(in.R, w->group));
+  const long long kept = (lm_kept(R, K) + 7) / 8 * 8;  // what follows is wider
+  auto keep = torch::empty({kept + n_rec + n_b + part * (rest ? 2 : 1) + n_xt + 1},
+                           x.options().dtype(torch::kFloat32).requires_grad(false));
+  *kp = lm_keep_of(keep, R, K);
+  float* at = keep.data_ptr<float>() + kept;
+  auto next = [&at](long long n) { float* p = at; at += n; return n ? p : nullptr; };
   w->rec = (double4*)next(n_rec);
-  w->bpart = (double2*)next(16LL * blocks);
+  w->bpart = (double2*)next(n_b);
   w->part = (float2*)next(part);
   w->part_top = (float2*)next(rest ? part : 0);
-  w->xt = (float*)next(n_xt);
-  w->counter = (int*)next(4);
-  return ws;
+  w->xt = next(n_xt);
+  w->counter = (int*)next(1);
+  return keep;
 }
 
 static torch::Tensor lm_loss_out(const torch::Tensor& x, at::IntArrayRef each,
@@ -693,10 +694,10 @@ static torch::Tensor lm_backward(AutogradContext* ctx, const torch::Tensor& grad
   const int64_t pairs = per == LM_UP_PAIR ? x.size(0) / 2 : 1;
   auto dx = torch::empty(x.sizes(), x.options().requires_grad(false));
   if (!R) return dx;
-  auto up = grad.to(torch::kFloat32).contiguous();
+  auto up = grad.scalar_type() == torch::kFloat32 && grad.is_contiguous()
+                ? grad : grad.to(torch::kFloat32).contiguous();
   lm_check_grid(in, lm_grad_splits(in));
-  float* f = keep.data_ptr<float>();
-  LmKeep kp{(LmStat*)f, f + 4 * R, f + 5 * R, K ? f + 5 * R + 1 : nullptr};
+  const LmKeep kp = lm_keep_of(keep, R, K);
   LmPlaces pl{};
   lm_set_idx(&pl, idx);
   pl.K = K ? (int)K : 1;
@@ -722,8 +723,8 @@ struct LmDistillFn : public torch::autograd::Function<LmDistillFn> {
     TORCH_CHECK(idx.device() == x.device() && values.device() == x.device(),
                 "distill: the record must be on the logits' device");
     c10::DeviceGuard guard(x.device());
-    idx = idx.contiguous();
-    values = values.contiguous();
+    if (!idx.is_contiguous()) idx = idx.contiguous();
+    if (!values.is_contiguous()) values = values.contiguous();
     if (lse) lse = lm_per_row(*lse, x, torch::kFloat32, "teacher_lse");
     if (mask) mask = lm_per_row(*mask, x, torch::kBool, "mask");
     LmPlaces pl{};
@@ -733,7 +734,8 @@ struct LmDistillFn : public torch::autograd::Function<LmDistillFn> {
     LmTeacher te{values.data_ptr(), (const float*)lm_ptr(lse),
                  lm_type(values, "teacher_values"), (float)temperature};
     LmKeep kp;
-    auto keep = lm_keep(x, in, pl.K, &kp);
+    LmWork w;
+    auto keep = lm_keep(x, in, pl.K, lse.has_value(), 0, &kp, &w);
     LmOut o;
     auto loss = lm_loss_out(x, rows, reduction, kp, &o);
     ctx->save_for_backward({x, idx, keep});
@@ -741,8 +743,6 @@ struct LmDistillFn : public torch::autograd::Function<LmDistillFn> {
     ctx->saved_data["t"] = temperature;
     ctx->saved_data["per"] = (int64_t)(reduction == LM_NONE ? LM_UP_ROW : LM_UP_ALL);
     if (!in.R) return loss.zero_();
-    LmWork w;
-    auto ws = lm_work(x, in, lse.has_value(), true, 0, &w);
     lm_distill(in, pl, te, w, kp, o, cur_stream());
     return loss;
   }
@@ -776,7 +776,8 @@ struct LmPolicyFn : public torch::autograd::Function<LmPolicyFn> {
     LmPolicy po{old_lp.data_ptr<float>(), adv.data_ptr<float>(),
                 (const float*)lm_ptr(ref_lp), clip_low, clip_high, kl_coef};
     LmKeep kp;
-    auto keep = lm_keep(x, in, 0, &kp);
+    LmWork w;
+    auto keep = lm_keep(x, in, 0, false, 0, &kp, &w);
     LmOut o;
     const auto rows = x.sizes().slice(0, x.dim() - 1);
     auto loss = lm_loss_out(x, rows, reduction, kp, &o);
@@ -787,8 +788,6 @@ struct LmPolicyFn : public torch::autograd::Function<LmPolicyFn> {
     ctx->mark_non_differentiable({logps, kl});
     ctx->set_materialize_grads(false);
     if (!in.R) return {loss.zero_(), logps, kl};
-    LmWork w;
-    auto ws = lm_work(x, in, false, false, 0, &w);
     lm_policy(in, pl, po, w, kp, logps.data_ptr<float>(), kl.data_ptr<float>(), o,
               cur_stream());
     return {loss, logps, kl};
@@ -813,8 +812,9 @@ struct LmPreferenceFn : public torch::autograd::Function<LmPreferenceFn> {
                 ref.size(0) == x.size(0), "preference: ref_logps must be [2N]");
     c10::DeviceGuard guard(x.device());
     targets = lm_per_row(targets, x, torch::kLong, "targets");
-    if (ref.scalar_type() != torch::kDouble) ref = ref.to(torch::kFloat32);
-    ref = ref.contiguous();
+    if (ref.scalar_type() != torch::kDouble && ref.scalar_type() != torch::kFloat32)
+      ref = ref.to(torch::kFloat32);
+    if (!ref.is_contiguous()) ref = ref.contiguous();
     LmPlaces pl{};
     lm_set_idx(&pl, targets);
     pl.K = 1;
@@ -824,7 +824,8 @@ struct LmPreferenceFn : public torch::autograd::Function<LmPreferenceFn> {
                     smoothing};
     const int64_t N = x.size(0) / 2;
     LmKeep kp;
-    auto keep = lm_keep(x, in, 0, &kp);
+    LmWork w;
+    auto keep = lm_keep(x, in, 0, false, (int)N, &kp, &w);
     LmOut o;
     auto loss = lm_loss_out(x, {N}, reduction, kp, &o);
     const auto opt = loss.options();
@@ -834,8 +835,6 @@ struct LmPreferenceFn : public torch::autograd::Function<LmPreferenceFn> {
     ctx->mark_non_differentiable({chosen, rejected});
     ctx->set_materialize_grads(false);
     if (!in.R) return {loss.zero_(), chosen, rejected};
-    LmWork w;
-    auto ws = lm_work(x, in, false, false, (int)N, &w);
     lm_preference(in, pl, pr, w, kp, chosen.data_ptr<float>(),
                   rejected.data_ptr<float>(), o, cur_stream());
     return {loss, chosen, rejected};

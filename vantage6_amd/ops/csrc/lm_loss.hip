@@ -172,26 +172,26 @@ DEVINL float wave_add(float v) {
 // finite float, so that -inf adds 0 and never meets itself in a difference.
 struct Run {
   float m, s;
-  DEVINL void join(float om, float os, float c) {
-    float mn = fmaxf(m, om);
-    s = s * exp2_hw((m - mn) * c) + os * exp2_hw((om - mn) * c);
+  DEVINL void join(float om, float os, const LmRows& in) {
+    const float mn = fmaxf(m, om);
+    s = s * exp_of(m - mn, in) + os * exp_of(om - mn, in);
     m = mn;
   }
 };
 DEVINL Run run_empty() { return {-FLT_MAX, 0.f}; }
-DEVINL Run wave_join(Run a, float c) {
+DEVINL Run wave_join(Run a, const LmRows& in) {
   const float m = wave_max(a.m);
-  return {m, wave_add(a.s * exp2_hw((a.m - m) * c))};
+  return {m, wave_add(a.s * exp_of(a.m - m, in))};
 }
 
 template <int THREADS>
-DEVINL Run block_join(Run a, float c, Run* red) {
-  a = wave_join(a, c);
+DEVINL Run block_join(Run a, const LmRows& in, Run* red) {
+  a = wave_join(a, in);
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = a;
   __syncthreads();
   a = red[0];
 #pragma unroll
-  for (int w = 1; w < THREADS / 64; ++w) a.join(red[w].m, red[w].s, c);
+  for (int w = 1; w < THREADS / 64; ++w) a.join(red[w].m, red[w].s, in);
   return a;
 }
 
@@ -361,7 +361,7 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
           for (int e = 0; e < X::N; ++e)
             if (hit >> e & 1) {
-              top.join(f[g * X::N + e], 1.f, c);
+              top.join(f[g * X::N + e], 1.f, in);
               f[g * X::N + e] = -INFINITY;
             }
         }
@@ -405,14 +405,14 @@ __global__ void __launch_bounds__(kThreads)
     int j = nv * X::N + tid;
     float f = X::one(x + (long long)j * X::size);
     if (TOP && (bits[j >> 5] >> (j & 31) & 1))
-      top.join(f, 1.f, c);
+      top.join(f, 1.f, in);
     else
-      a.join(f, 1.f, c);
+      a.join(f, 1.f, in);
   }
-  a = block_join<kThreads>(a, c, red);
+  a = block_join<kThreads>(a, in, red);
   if (TOP) {
     __syncthreads();
-    top = block_join<kThreads>(top, c, red);
+    top = block_join<kThreads>(top, in, red);
   }
   if (tid == 0) {
     const long long at = (long long)r * splits + sp;
@@ -844,9 +844,9 @@ __global__ void __launch_bounds__(THREADS)
   if (tid < left) {
     const float f = X::one(x + (long long)(nv * X::N + tid) * X::size);
     if (PIECE == kLogits) maxima[nv * X::N + tid] = f;
-    a.join(f, 1.f, c);
+    a.join(f, 1.f, in);
   }
-  a = wave_join(a, c);
+  a = wave_join(a, in);
   if ((tid & 63) == 0) red[tid >> 6] = a;
   __syncthreads();
   if (tid < 64) {
@@ -903,7 +903,7 @@ __global__ void __launch_bounds__(THREADS)
     // meanwhile another wave joins the sums
     constexpr int W = THREADS / 64;
     a = (tid & 63) < W ? red[tid & 63] : run_empty();
-    a = wave_join(a, c);
+    a = wave_join(a, in);
     if (tid == 64) {
       s_run = a;
       odd = a.s != a.s;  // a NaN hides from fmaxf, but not from the sum
@@ -1144,7 +1144,8 @@ int lm_group(int splits) {
 // are a few hundred.
 static int finish_threads(int R, int group) {
   const long long lanes = (long long)R * group;
-  return lanes <= kThreads ? (int)(lanes + 63) / 64 * 64 : lanes <= 16384 ? 64 : kThreads;
+  if (lanes <= kThreads) return std::max(64, (int)(lanes + 63) / 64 * 64);
+  return lanes <= 16384 ? 64 : kThreads;
 }
 
 int lm_finish_blocks(int R, int group) {

@@ -24,7 +24,7 @@ from typing import NamedTuple
 import torch
 
 from . import hip_ops
-from .lm_logits import (check_constant, check_logits, check_mask,
+from .lm_logits import (check_logits, check_mask,
                         check_reduction, check_rows, check_temperature, fold,
                         kernel_rows, reduce_rows, reference_dtype)
 
@@ -89,15 +89,13 @@ def distill_loss(logits: torch.Tensor, teacher_values: torch.Tensor,
     k = teacher_indices.shape[-1] if teacher_indices.dim() else 0
     if not 1 <= k <= MOST_K:
         raise ValueError(f"a record has between 1 and {MOST_K} entries, got {k}")
-    shape = (*logits.shape[:-1], k)
-    check_rows("teacher_indices", teacher_indices, logits, shape=shape, floating=False)
-    check_rows("teacher_values", teacher_values, logits, shape=shape, floating=True)
-    check_constant("teacher_values", teacher_values)
+    rows = logits.shape[:-1]
+    check_rows("teacher_indices", teacher_indices, logits, (*rows, k), False)
+    check_rows("teacher_values", teacher_values, logits, (*rows, k), True)
     if teacher_lse is not None:
-        check_rows("teacher_lse", teacher_lse, logits, floating=True)
-        check_constant("teacher_lse", teacher_lse)
+        check_rows("teacher_lse", teacher_lse, logits, rows, True)
     if mask is not None:
-        check_mask(mask, logits)
+        check_mask(mask, logits, rows)
     if logits.is_cuda:
         if teacher_values.dtype == torch.float64:
             teacher_values = teacher_values.float()
@@ -105,7 +103,7 @@ def distill_loss(logits: torch.Tensor, teacher_values: torch.Tensor,
         loss = hip_ops().lm_distill_loss(
             x, fold(teacher_values, x, 1), fold(teacher_indices, x, 1),
             fold(teacher_lse, x), temperature, fold(mask, x), red)
-        return loss.reshape(logits.shape[:-1]) if reduction == "none" else loss
+        return loss.reshape(rows) if reduction == "none" else loss
     return _distill_reference(logits, teacher_values, teacher_indices,
                               teacher_lse, temperature, mask, reduction)
 

@@ -24,30 +24,28 @@ def check_logits(logits: torch.Tensor) -> None:
                          f"(float64 on the CPU alone), got {logits.dtype}")
 
 
-def check_rows(name: str, t: torch.Tensor, logits: torch.Tensor, *,
-               shape=None, floating: bool | None = None) -> None:
-    """``t`` has one value per row of ``logits`` (or ``shape``), on its device."""
-    want = tuple(logits.shape[:-1]) if shape is None else tuple(shape)
-    if tuple(t.shape) != want:
-        raise ValueError(f"{name} must have shape {want}, got {tuple(t.shape)}")
+def check_rows(name: str, t: torch.Tensor, logits: torch.Tensor, want,
+               floating: bool | None = None) -> None:
+    """``t`` has the shape ``want`` (the rows' or more), on the logits' device;
+    of floats, or (``floating`` False) of int64 or int32."""
+    if t.shape != want:
+        raise ValueError(f"{name} must have shape {tuple(want)}, got {tuple(t.shape)}")
     if t.device != logits.device:
         raise ValueError(f"{name} is on {t.device}, logits on {logits.device}")
-    if floating is True and not t.is_floating_point():
-        raise ValueError(f"{name} must be floating point, got {t.dtype}")
-    if floating is False and t.dtype not in (torch.int64, torch.int32):
+    if floating:
+        if not t.is_floating_point():
+            raise ValueError(f"{name} must be floating point, got {t.dtype}")
+        if t.requires_grad and torch.is_grad_enabled():
+            # not to drop a gradient that the caller may expect
+            raise ValueError(f"{name} is a constant of this loss: detach it")
+    elif floating is False and t.dtype not in (torch.int64, torch.int32):
         raise ValueError(f"{name} must be int64 or int32, got {t.dtype}")
 
 
-def check_constant(name: str, t: torch.Tensor) -> None:
-    """Refuse to drop a gradient that the caller may expect."""
-    if t.requires_grad and torch.is_grad_enabled():
-        raise ValueError(f"{name} is a constant of this loss: detach it")
-
-
-def check_mask(mask: torch.Tensor, logits: torch.Tensor) -> None:
+def check_mask(mask: torch.Tensor, logits: torch.Tensor, want) -> None:
     if mask.dtype != torch.bool:
         raise ValueError(f"mask must be bool, got {mask.dtype}")
-    check_rows("mask", mask, logits)
+    check_rows("mask", mask, logits, want)
 
 
 def check_reduction(reduction: str) -> int:

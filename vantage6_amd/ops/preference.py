@@ -23,9 +23,8 @@ from typing import NamedTuple
 import torch
 
 from . import hip_ops
-from .lm_logits import (check_constant, check_logits,
-                        check_mask, check_reduction, check_rows, fold,
-                        kernel_rows, reduce_rows, reference_dtype)
+from .lm_logits import (check_logits, check_mask, check_reduction, check_rows,
+                        fold, kernel_rows, reduce_rows, reference_dtype)
 
 
 class PreferenceLoss(NamedTuple):
@@ -71,9 +70,8 @@ def preference_loss(logits: torch.Tensor, targets: torch.Tensor,
                          f"{tuple(logits.shape)}")
     if logits.shape[0] and not logits.shape[1]:
         raise ValueError("answers must have at least one position")
-    check_rows("targets", targets, logits, floating=False)
-    check_rows("ref_logps", ref_logps, logits, shape=logits.shape[:1], floating=True)
-    check_constant("ref_logps", ref_logps)
+    check_rows("targets", targets, logits, logits.shape[:2], False)
+    check_rows("ref_logps", ref_logps, logits, logits.shape[:1], True)
     if not (math.isfinite(beta) and beta > 0):
         raise ValueError(f"beta must be positive, got {beta}")
     if not 0 <= label_smoothing < 0.5:
@@ -115,14 +113,14 @@ def policy_loss(logits: torch.Tensor, actions: torch.Tensor,
     ``reduction``: "mean" over the tokens that count, "sum", or "none"."""
     check_logits(logits)
     red = check_reduction(reduction)
-    check_rows("actions", actions, logits, floating=False)
-    for name, t in (("old_logps", old_logps), ("advantages", advantages),
-                    ("ref_logps", ref_logps)):
-        if t is not None:
-            check_rows(name, t, logits, floating=True)
-            check_constant(name, t)
+    shape = logits.shape[:-1]
+    check_rows("actions", actions, logits, shape, False)
+    check_rows("old_logps", old_logps, logits, shape, True)
+    check_rows("advantages", advantages, logits, shape, True)
+    if ref_logps is not None:
+        check_rows("ref_logps", ref_logps, logits, shape, True)
     if mask is not None:
-        check_mask(mask, logits)
+        check_mask(mask, logits, shape)
     if not 0 <= clip_low < 1 or not (math.isfinite(clip_high) and clip_high >= 0):
         raise ValueError("clip_low must be in [0, 1) and clip_high >= 0, got "
                          f"{clip_low}, {clip_high}")
@@ -136,9 +134,8 @@ def policy_loss(logits: torch.Tensor, actions: torch.Tensor,
             x, fold(actions, x), fold(old_logps, x), fold(advantages, x),
             fold(ref_logps, x), fold(mask, x), clip_low, clip_high, kl_coef, red)
         if x.dim() != logits.dim():
-            rows = logits.shape[:-1]
-            logps, kl = logps.reshape(rows), kl.reshape(rows)
-            loss = loss.reshape(rows) if reduction == "none" else loss
+            logps, kl = logps.reshape(shape), kl.reshape(shape)
+            loss = loss.reshape(shape) if reduction == "none" else loss
         return PolicyLoss(loss, logps, kl)
     live = torch.ones_like(actions, dtype=torch.bool) if mask is None else mask
     lp = _token_logps(logits, actions.long(), live)
