@@ -27,6 +27,11 @@ from vantage6_amd.parallel.fedavg import FedAvgConfig, FedAvgTrainer
 # --------------------------------------------------------------------------
 # shared helpers
 # --------------------------------------------------------------------------
+# what another model or a rollout measured: compared with, not computed in
+_EXACT_KEYS = frozenset(("teacher_values", "teacher_lse", "ref_logps",
+                         "old_logps", "advantages"))
+
+
 def make_batches(dataset: dict, batch_size: int, device, dtype=torch.bfloat16,
                  seed: int = 0):
     """Infinite minibatch iterator over a resident synthetic/tensor shard."""
@@ -35,7 +40,7 @@ def make_batches(dataset: dict, batch_size: int, device, dtype=torch.bfloat16,
     g = torch.Generator().manual_seed(seed)
 
     def to_dev(t, k):
-        if t.is_floating_point():
+        if t.is_floating_point() and k not in _EXACT_KEYS:
             return t.to(device=device, dtype=dtype)
         return t.to(device=device)
 
@@ -45,10 +50,11 @@ def make_batches(dataset: dict, batch_size: int, device, dtype=torch.bfloat16,
         yield {k: v[idx] for k, v in resident.items()}
 
 
-def _build(model_name: str, model_kwargs: dict, device, seed: int = 1234):
+def _build(model_name: str, model_kwargs: dict, device, seed: int = 1234,
+           objective: str | None = None, objective_options: dict | None = None):
     torch.manual_seed(seed)  # identical init across stations
     model = build_model(model_name, device=device, **(model_kwargs or {}))
-    return model, model_loss(model_name)
+    return model, model_loss(model_name, objective, **(objective_options or {}))
 
 
 # --------------------------------------------------------------------------
@@ -77,14 +83,22 @@ def fit_rounds(
     round_hook=None,
     checkpoint: str | None = None,
     checkpoint_every: int = 0,
+    objective: str | None = None,
+    objective_options: dict | None = None,
 ) -> dict:
-    """Engine mode. With ``checkpoint`` set, training resumes from the file
+    """Engine mode. ``objective`` ("distill", "preference", "policy") trains a
+    language model on something else than its next token; ``dataset`` then
+    holds what ``models.model_loss`` names for it. With ``checkpoint`` set, training resumes from the file
     if it exists and (with ``checkpoint_every`` > 0) saves every N rounds —
     the reference's long-running-task recovery story on
     the engine path."""
     comm = comm or init_from_env()
     device = device or comm.device
-    net, loss_fn = _build(model, model_kwargs, device)
+    if dp and objective is not None:
+        raise ValueError("DP-SGD clips per-sample next-token losses only: no "
+                         f"objective {objective!r}")
+    net, loss_fn = _build(model, model_kwargs, device, objective=objective,
+                          objective_options=objective_options)
     batches = make_batches(dataset, batch_size, device, seed=17 + comm.rank)
     dp_cfg = None
     if dp:

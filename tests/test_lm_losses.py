@@ -871,3 +871,147 @@ def test_station_learns_from_a_record(device, tail):
                             temperature=2.0)
     slope = (grad * grad).sum().item()
     assert down.item() < loss.item() - 0.5 * 1e-2 * slope
+
+
+# ------------------------------------------------------------ through the engine
+TINY = {
+    "llama_1b": dict(vocab=131, hidden=64, layers=1, heads=1, kv_heads=1, ffn=128),
+    # a head padded to 56 columns, of which 50 are real
+    "bert_base": dict(vocab=50, hidden=64, layers=1, heads=1, ffn=64, max_seq=16, vocab_pad=56),
+}
+
+
+def objective_data(model, vocab, objective, n=6, S=8, seed=0):
+    """A dataset as a station holds it, on the CPU."""
+    from vantage6_amd.models import teacher_record
+
+    g = torch.Generator().manual_seed(seed)
+    if objective == "preference":
+        mask = torch.ones(n, 2, S, dtype=torch.bool)
+        mask[:, :, :3] = False
+        return {"input_ids": torch.randint(0, vocab, (n, 2, S), generator=g), "mask": mask,
+                "ref_logps": torch.randn(n, 2, generator=g) - 20.0}
+    data = {"input_ids": torch.randint(0, vocab, (n, S), generator=g)}
+    data["mask"] = torch.arange(S)[None] < torch.randint(3, S + 1, (n, 1), generator=g)
+    if objective == "distill":
+        device = next(model.parameters()).device
+        record = teacher_record(model, data["input_ids"].to(device), 5, 2.0)
+        assert (record["teacher_indices"] < vocab).all()
+        return {**data, **{k: v.cpu() for k, v in record.items()}}
+    data["old_logps"] = torch.randn(n, S - 1, generator=g) * 0.1 - math.log(vocab)
+    data["ref_logps"] = torch.randn(n, S - 1, generator=g) * 0.1 - math.log(vocab)
+    data["advantages"] = torch.randn(n, S - 1, generator=g)
+    return data
+
+
+OPTIONS = {"distill": {"temperature": 2.0}, "preference": {"beta": 0.2},
+           "policy": {"kl_coef": 0.1, "clip_high": 0.3}}
+
+
+@pytest.mark.parametrize("device", CPU_GPU)
+@pytest.mark.parametrize("name", list(TINY))
+@pytest.mark.parametrize("objective", list(OPTIONS))
+def test_objectives_of_the_models(device, name, objective):
+    """The factory's objective is the loss on the model's own logits, and its
+    gradient reaches every weight."""
+    need(device)
+    from vantage6_amd.models import build_model, model_loss
+
+    torch.manual_seed(0)
+    dtype = torch.bfloat16 if device == "cuda" else torch.float32
+    model = build_model(name, dtype=dtype, device=device, **TINY[name])
+    vocab = TINY[name]["vocab"]
+    batch = {k: v.to(device) for k, v in objective_data(model, vocab, objective).items()}
+    if objective == "distill":
+        batch["teacher_values"] = batch["teacher_values"] * 1.5  # not the model's own
+    loss = model_loss(name, objective, **OPTIONS[objective])(model, batch)
+    loss.backward()
+    assert all(p.grad is not None and torch.isfinite(p.grad).all() for p in model.parameters())
+    assert model.head.weight.grad[:vocab].abs().sum() > 0
+    assert (model.head.weight.grad[vocab:] == 0).all()
+    with torch.no_grad():
+        ids = batch["input_ids"]
+        if objective == "distill":
+            rows, live, _ = distill_oracle(model(ids)[..., :vocab], batch["teacher_values"],
+                                           batch["teacher_indices"], batch["teacher_lse"], 2.0,
+                                           batch["mask"])
+            want = rows.sum() / live.sum()
+        elif objective == "preference":
+            both = torch.cat([ids[:, 0], ids[:, 1]])
+            targets = both[:, 1:].masked_fill(
+                ~torch.cat([batch["mask"][:, 0], batch["mask"][:, 1]])[:, 1:], -100)
+            ref = torch.cat([batch["ref_logps"][:, 0], batch["ref_logps"][:, 1]])
+            want = preference_oracle(model(both[:, :-1])[..., :vocab], targets, ref, 0.2, 0.0,
+                                     -100)[0].mean()
+        else:
+            rows, *_, live = policy_oracle(model(ids[:, :-1])[..., :vocab], ids[:, 1:],
+                                           batch["old_logps"], batch["advantages"],
+                                           batch["ref_logps"], batch["mask"][:, 1:], 0.2, 0.3, 0.1)
+            want = rows.sum() / live.sum()
+    # the same logits twice, one loss: its own error
+    assert abs(loss.item() - want.item()) <= 50 * LP + 2.0 ** -22 * abs(want.item())
+
+
+@pytest.mark.parametrize("device", CPU_GPU)
+@pytest.mark.parametrize("objective", list(OPTIONS))
+def test_fit_rounds_with_an_objective(device, objective):
+    need(device)
+    from algorithms.fedavg import fit_rounds, make_batches
+    from vantage6_amd.models import build_model
+
+    torch.manual_seed(1)
+    kw = dict(TINY["llama_1b"])
+    teacher = build_model("llama_1b", device=device, **kw)
+    data = objective_data(teacher, kw["vocab"], objective)
+    out = fit_rounds(data, model="llama_1b", model_kwargs=kw, rounds=2, local_steps=2,
+                     batch_size=4, lr=0.01, device=torch.device(device), objective=objective,
+                     objective_options=OPTIONS[objective])
+    assert out["rounds"] == 2 and all(math.isfinite(h["loss"]) for h in out["history"])
+    batch = next(make_batches(data, 4, device))
+    assert all(batch[k].dtype == data[k].dtype for k in data)  # measured values stay exact
+
+
+def test_objective_refusals():
+    from algorithms.fedavg import fit_rounds
+    from vantage6_amd.models import model_loss
+
+    for call in (lambda: model_loss("resnet18", "distill"), lambda: model_loss("llama_1b", "lm"),
+                 lambda: model_loss("llama_1b", temperature=2.0),
+                 lambda: fit_rounds({"input_ids": torch.zeros(2, 4, dtype=torch.int64)},
+                                    model="llama_1b", dp={"max_grad_norm": 1.0}, objective="policy",
+                                    device=torch.device("cpu"))):
+        with pytest.raises(ValueError):
+            call()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("objective", list(OPTIONS))
+def test_objective_in_a_captured_step(objective):
+    """The trainer's captured local step, replayed, against eager steps: the
+    same losses, bit for bit."""
+    need("cuda")
+    from algorithms.fedavg import _build, make_batches
+    from vantage6_amd.models import build_model
+    from vantage6_amd.parallel.comm import CommContext
+    from vantage6_amd.parallel.fedavg import FedAvgConfig, FedAvgTrainer
+
+    kw, dev = TINY["llama_1b"], torch.device("cuda", 0)
+    torch.manual_seed(1)
+    data = objective_data(build_model("llama_1b", device=dev, **kw), kw["vocab"], objective)
+    losses = []
+    for graph in (False, True):
+        net, loss_fn = _build("llama_1b", kw, dev, objective=objective,
+                              objective_options=OPTIONS[objective])
+        # the same batch each time, whatever the capture draws
+        fixed = next(make_batches(data, 4, dev))
+
+        def batches():
+            while True:
+                yield fixed
+
+        trainer = FedAvgTrainer(net, loss_fn, batches(), CommContext(device=dev),
+                                FedAvgConfig(local_steps=1, lr=0.01), n_samples=6)
+        if graph:
+            assert trainer.enable_graph()
+        losses.append([trainer.local_step() for _ in range(5)])
+    assert losses[0] == losses[1] and len(set(losses[0])) > 1

@@ -10,4 +10,4 @@ All models run in bf16 with our hand-written ops on the hot path
 ships no models at all (compute lives in user Docker images),
 so this zoo is part of the net-new MI355X compute plane.
 """
-from .factory import build_model, model_loss  # noqa: F401
+from .factory import build_model, model_loss, teacher_record  # noqa: F401

@@ -36,11 +36,96 @@ def build_model(name: str, device="cpu", dtype=torch.bfloat16, **kw) -> torch.nn
     raise ValueError(f"unknown model {name!r}")
 
 
-def model_loss(name: str) -> Callable:
-    """(model, batch) -> scalar loss, fp32 loss computation."""
+_LM_NAMES = ("bert", "bert_base", "bert-base", "llama", "llama_1b", "llama-1b",
+             "llama-3-1b")
+
+
+def _lm_logits(model, ids):
+    """Logits over the real vocabulary: a padded head's extra columns are cut
+    off as a view, which the losses over logits read in place."""
+    logits = model(ids)
+    vl = getattr(model, "vocab_logical", logits.shape[-1])
+    return logits[..., :vl] if vl < logits.shape[-1] else logits
+
+
+def _distill_objective(options) -> Callable:
+    """Batch: ``input_ids`` [N, S] and the teacher's record of every position,
+    ``teacher_values`` and ``teacher_indices`` [N, S, k], optionally
+    ``teacher_lse`` and ``mask`` [N, S]."""
+    def loss(model, batch):
+        from ..ops.distill import distill_loss
+
+        return distill_loss(
+            _lm_logits(model, batch["input_ids"]), batch["teacher_values"],
+            batch["teacher_indices"], batch.get("teacher_lse"),
+            mask=batch.get("mask"), **options)
+
+    return loss
+
+
+def _preference_objective(options) -> Callable:
+    """Batch: ``input_ids`` [N, 2, S] (chosen, rejected), ``ref_logps`` [N, 2],
+    optionally ``mask`` [N, 2, S], True where a token is one of the answer."""
+    def loss(model, batch):
+        from ..ops.preference import preference_loss
+
+        ids = batch["input_ids"].transpose(0, 1).flatten(0, 1)
+        targets = ids[:, 1:]
+        if "mask" in batch:
+            mask = batch["mask"].transpose(0, 1).flatten(0, 1)[:, 1:]
+            targets = torch.where(mask, targets, -100)
+        ref = batch["ref_logps"].transpose(0, 1).flatten()
+        return preference_loss(_lm_logits(model, ids[:, :-1]), targets, ref,
+                               **options).loss
+
+    return loss
+
+
+def _policy_objective(options) -> Callable:
+    """Batch: ``input_ids`` [N, S]; of the tokens that its positions 1.. hold,
+    ``old_logps``, ``advantages`` and optionally ``ref_logps`` [N, S - 1];
+    optionally ``mask`` [N, S], True where a token was sampled."""
+    def loss(model, batch):
+        from ..ops.preference import policy_loss
+
+        ids = batch["input_ids"]
+        mask = batch["mask"][:, 1:] if "mask" in batch else None
+        return policy_loss(_lm_logits(model, ids[:, :-1]), ids[:, 1:],
+                           batch["old_logps"], batch["advantages"],
+                           batch.get("ref_logps"), mask=mask, **options).loss
+
+    return loss
+
+
+_OBJECTIVES = {"distill": _distill_objective, "preference": _preference_objective,
+               "policy": _policy_objective}
+
+
+@torch.no_grad()
+def teacher_record(model, input_ids, k: int = 64, temperature: float = 1.0) -> dict:
+    """What a station publishes of its model's answers to ``input_ids``: the
+    entries that the "distill" objective's batches hold."""
+    from ..ops.distill import topk_logits
+
+    top = topk_logits(_lm_logits(model, input_ids), k, temperature)
+    return {"teacher_values": top.values, "teacher_indices": top.indices,
+            "teacher_lse": top.logsumexp}
+
+
+def model_loss(name: str, objective: str | None = None, **options) -> Callable:
+    """(model, batch) -> scalar loss, fp32 loss computation.
+
+    Language models take an ``objective`` other than the next token:
+    "distill", "preference" or "policy", with ``options`` for its loss
+    (``temperature``, ``beta``, ``kl_coef``, ...)."""
     name = name.lower()
-    if name in ("bert", "bert_base", "bert-base", "llama", "llama_1b", "llama-1b",
-                "llama-3-1b"):
+    if objective is not None:
+        if name not in _LM_NAMES or objective not in _OBJECTIVES:
+            raise ValueError(f"no objective {objective!r} for model {name!r}")
+        return _OBJECTIVES[objective](options)
+    if options:
+        raise ValueError(f"options {sorted(options)} need an objective")
+    if name in _LM_NAMES:
 
         def lm_loss(model, batch):
             from ..ops.cross_entropy import cross_entropy
@@ -67,8 +152,7 @@ def model_loss(name: str) -> Callable:
 def model_loss_per_sample(name: str) -> Callable:
     """(model, batch) -> per-sample loss vector [B] (DP-SGD needs this)."""
     name = name.lower()
-    if name in ("bert", "bert_base", "bert-base", "llama", "llama_1b", "llama-1b",
-                "llama-3-1b"):
+    if name in _LM_NAMES:
 
         def lm_loss_ps(model, batch):
             from ..ops.cross_entropy import cross_entropy
