@@ -436,6 +436,22 @@ def test_preference_far_margins(device):
 
 
 @pytest.mark.parametrize("device", CPU_GPU)
+def test_preference_impossible_answers(device):
+    """A token whose logit is -inf: an impossible rejected answer costs
+    nothing, an impossible chosen one everything, and neither is a NaN."""
+    need(device)
+    x = make_logits(4, 3, 64, torch.float32, device)
+    x[[1, 2], 1, 5] = float("-inf")
+    x.requires_grad_(True)
+    targets = torch.full((4, 3), 5, device=device)
+    out = preference_loss(x, targets, torch.zeros(4, device=device), reduction="none")
+    assert out.loss.tolist() == [0.0, math.inf]
+    assert out.rejected_rewards[0].item() == out.chosen_rewards[1].item() == -math.inf
+    grad, = torch.autograd.grad(out.loss.sum(), x)
+    assert (grad[[0, 2]] == 0).all() and torch.isfinite(grad[3]).all() and grad[3].abs().sum() > 0
+
+
+@pytest.mark.parametrize("device", CPU_GPU)
 def test_preference_target_outside_is_nan(device):
     need(device)
     x = make_logits(4, 3, 64, torch.float32, device).requires_grad_(True)

@@ -200,15 +200,18 @@ DEVINL double wave_sum(double v) {
   for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
   return v;
 }
-// the sum over a block in every thread, in one order
-DEVINL double block_sum(double v, double* red) {
-  v = wave_sum(v);
+// two sums over a block in every thread, in one order
+DEVINL void block_sum2(double& a, double& b, double2* red) {
+  a = wave_sum(a);
+  b = wave_sum(b);
   __syncthreads();
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = make_double2(a, b);
   __syncthreads();
-  v = 0.0;
-  for (int w = 0; w < (int)(blockDim.x >> 6); ++w) v += red[w];
-  return v;
+  a = b = 0.0;
+  for (int w = 0; w < (int)(blockDim.x >> 6); ++w) {
+    a += red[w].x;
+    b += red[w].y;
+  }
 }
 
 // A record's probabilities by one wave, up to 4 of its 256 entries a lane, in
@@ -448,15 +451,14 @@ DEVINL Row join_splits(const float2* part, int splits, int group, int r,
   return {(double)m, s};
 }
 
-// Sum of `loss` and `count` over the whole grid, in one order: each block's
-// sums in memory, the block that arrives last adds them up. *o.loss = the loss,
-// *o.inv = 1/count for a mean over the rows that count, else 1.
+// Sum over the whole grid of a block's `loss` and `count`, as its first thread
+// has them, in one order: each block's sums in memory, the block that arrives
+// last adds them up. *o.loss = the loss, *o.inv = 1/count for a mean over what
+// counts, else 1.
 DEVINL void grid_mean(double loss, double count, double2* bpart, int* counter,
                       const LmOut& o) {
-  __shared__ double red[16];
+  __shared__ double2 red[16];
   __shared__ int last;
-  loss = block_sum(loss, red);
-  count = block_sum(count, red);
   if (gridDim.x > 1) {
     if (threadIdx.x == 0) {
       bpart[blockIdx.x] = make_double2(loss, count);
@@ -473,14 +475,24 @@ DEVINL void grid_mean(double loss, double count, double2* bpart, int* counter,
       count += __hip_atomic_load(&bpart[i].y, __ATOMIC_RELAXED,
                                  __HIP_MEMORY_SCOPE_AGENT);
     }
-    loss = block_sum(loss, red);
-    count = block_sum(count, red);
+    block_sum2(loss, count, red);
   }
   if (threadIdx.x == 0) {
     const double inv = o.reduction == LM_MEAN ? 1.0 / fmax(count, 1.0) : 1.0;
     *o.loss = (float)(loss * inv);
     *o.inv = (float)inv;
   }
+}
+
+// The same of a row's loss per lane that leads one.
+DEVINL void grid_mean_of_rows(double loss, bool lead, bool live, const LmWork& w,
+                              const LmOut& o) {
+  __shared__ double2 red[16];
+  if (o.reduction == LM_NONE) return;
+  double count = lead && live ? 1.0 : 0.0;
+  loss = lead ? loss : 0.0;
+  block_sum2(loss, count, red);
+  grid_mean(loss, count, w.bpart, w.counter, o);
 }
 
 // ------------------------------------------------------------------ distill
@@ -530,8 +542,7 @@ __global__ void __launch_bounds__(kThreads)
     kp.coef[r] = a;
     if (o.reduction == LM_NONE) o.loss[r] = (float)loss;
   }
-  if (o.reduction != LM_NONE)
-    grid_mean(lead ? loss : 0.0, lead && live ? 1.0 : 0.0, w.bpart, w.counter, o);
+  grid_mean_of_rows(loss, lead, live, w, o);
 }
 
 // ------------------------------------------- log-probability of one token
@@ -577,8 +588,7 @@ __global__ void __launch_bounds__(kThreads)
     kls[r] = (float)kl;
     if (o.reduction == LM_NONE) o.loss[r] = (float)loss;
   }
-  if (o.reduction != LM_NONE)
-    grid_mean(lead ? loss : 0.0, lead && live ? 1.0 : 0.0, w.bpart, w.counter, o);
+  grid_mean_of_rows(loss, lead, live, w, o);
 }
 
 // One block per pair: sequences n and n + N. The sums over an answer are held
@@ -587,7 +597,8 @@ __global__ void __launch_bounds__(1024)
     lm_preference_kernel(LmRows in, LmPlaces pl, LmPreference pr, LmWork w,
                          LmKeep kp, float* __restrict__ chosen,
                          float* __restrict__ rejected, LmOut o) {
-  __shared__ double red[16];
+  __shared__ double2 red[16];
+  __shared__ float s_a;
   const int n = blockIdx.x, N = gridDim.x, T = in.T;
   const int mine = threadIdx.x / w.group, rows = blockDim.x / w.group;
   const bool lead = (threadIdx.x & (w.group - 1)) == 0;
@@ -604,36 +615,35 @@ __global__ void __launch_bounds__(1024)
       sum[1] += side ? lp : 0.0;
     }
   }
-  sum[0] = block_sum(sum[0], red);
-  sum[1] = block_sum(sum[1], red);
-  double reward[2];
-#pragma unroll
-  for (int side = 0; side < 2; ++side) {
-    const int b = n + side * N;
-    const double ref = pr.ref64 ? ((const double*)pr.ref)[b]
-                                : (double)((const float*)pr.ref)[b];
-    reward[side] = pr.beta * (sum[side] - ref);
-  }
-  const double z = reward[0] - reward[1], e = pr.smoothing;
-  const double softplus = fmax(z, 0.0) + log1p(exp(-fabs(z)));
-  double loss = (1.0 - e) * (softplus - z) + e * softplus;
-  if (z != z) loss = z;
-  const double by_z = 1.0 / (1.0 + exp(-z)) - (1.0 - e);
-#pragma unroll
-  for (int side = 0; side < 2; ++side) {
-    const int r0 = (n + side * N) * T;
-    const float a = (float)((side ? 1.0 : -1.0) * pr.beta * by_z);
-    for (int t = threadIdx.x; t < T; t += blockDim.x)
-      kp.coef[r0 + t] = ignored(pl, r0 + t) ? 0.f : a;
-  }
+  block_sum2(sum[0], sum[1], red);
+  double loss = 0.0;
   if (threadIdx.x == 0) {
+    double reward[2];
+#pragma unroll
+    for (int side = 0; side < 2; ++side) {
+      const int b = n + side * N;
+      const double ref = pr.ref64 ? ((const double*)pr.ref)[b]
+                                  : (double)((const float*)pr.ref)[b];
+      reward[side] = pr.beta * (sum[side] - ref);
+    }
+    // -log sigmoid(z) = max(-z, 0) + log(1 + exp(-|z|))
+    const double z = reward[0] - reward[1], e = pr.smoothing;
+    const double both = log1p(exp(-fabs(z)));
+    loss = (1.0 - e) * (fmax(-z, 0.0) + both);
+    if (e != 0.0) loss += e * (fmax(z, 0.0) + both);
+    s_a = (float)(pr.beta * (1.0 - e - 1.0 / (1.0 + exp(-z))));
     chosen[n] = (float)reward[0];
     rejected[n] = (float)reward[1];
     if (o.reduction == LM_NONE) o.loss[n] = (float)loss;
   }
-  if (o.reduction != LM_NONE)
-    grid_mean(threadIdx.x == 0 ? loss : 0.0, threadIdx.x == 0 ? 1.0 : 0.0,
-              w.bpart, w.counter, o);
+  __syncthreads();
+  // the gradient is coef * (q - onehot), and the other way for the rejected
+  const float a = s_a;
+  for (int t = threadIdx.x; t < 2 * T; t += blockDim.x) {
+    const int side = t >= T, r = (n + side * N) * T + t - side * T;
+    kp.coef[r] = ignored(pl, r) ? 0.f : side ? -a : a;
+  }
+  if (o.reduction != LM_NONE) grid_mean(loss, 1.0, w.bpart, w.counter, o);
 }
 
 // --------------------------------------------------------------------- grad
@@ -1040,9 +1050,9 @@ long long bytes_of(const LmRows& in) {
 
 constexpr int kStatBlocks = 1024, kStatSeg = 131072;
 constexpr int kGradBlocks = 2048, kGradSeg = 32768;
-// Blocks of 512 threads cost the same at 1024 rows of 128256 (56 us), those of
-// 256 more (64).
-constexpr int kTopkThreads = 1024;
+// At 1024 rows of 128256 blocks of 1024 threads take as long (56 us) and those
+// of 256 longer (64); at 4000 rows of 8000 512 take 44 us, 1024 take 72.
+constexpr int kTopkThreads = 512;
 
 // What the pass over a row leaves in the 256 MB cache behind the L2, the pass
 // of the gradient need not fetch again. At 525 MB of logits a cache that every

@@ -85,8 +85,9 @@ def preference_loss(logits: torch.Tensor, targets: torch.Tensor,
     lp = _token_logps(logits, targets, targets != ignore_index)
     r = beta * (lp.sum(-1) - ref_logps.double())
     z = r[:n] - r[n:]
-    rows = -((1 - label_smoothing) * torch.nn.functional.logsigmoid(z)
-             + label_smoothing * torch.nn.functional.logsigmoid(-z))
+    rows = -(1 - label_smoothing) * torch.nn.functional.logsigmoid(z)
+    if label_smoothing:
+        rows = rows - label_smoothing * torch.nn.functional.logsigmoid(-z)
     loss = reduce_rows(rows, None, reduction)
     if logits.dtype != torch.float64:
         loss = loss.float()
