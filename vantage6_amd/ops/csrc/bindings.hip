@@ -572,7 +572,7 @@ static LmRows lm_rows(const torch::Tensor& x, double temperature) {
   TORCH_CHECK(x.dim() >= 1 && x.dim() <= 3, "logits must be [V], [T, V] or [B, T, V]");
   const int64_t d = x.dim(), V = x.size(d - 1);
   const int64_t T = d > 1 ? x.size(d - 2) : 1, B = d > 2 ? x.size(0) : 1;
-  TORCH_CHECK(V >= 1 && V < (1LL << 30), "logits: unsupported vocabulary size");
+  TORCH_CHECK(V >= 1 && V < (1LL << 28), "logits: unsupported vocabulary size");
   TORCH_CHECK(V == 1 || x.stride(d - 1) == 1, "logits of a row must be contiguous");
   TORCH_CHECK(B * T < (1LL << 22), "logits: at most 4194303 rows a call");
   LmRows in;

@@ -126,6 +126,27 @@ DEVINL bool ignored(const LmPlaces& pl, int r) {
          (pl.use_ignore && place(pl, r) == pl.ignore);
 }
 
+// A stretch of n elements at p as vectors that begin where a cache line does,
+// and up to 70 loose elements before and behind them. A wave's store of 1 KB
+// then covers whole lines: the gradient of 4096 rows of 30522 fp16 logits, which
+// begin anywhere in a line, took 68 us in vectors from each row's start and takes
+// 56, that of rows of 30521 76 and 56.
+struct Cut {
+  int head, nv, loose;
+};
+template <int TY>
+DEVINL Cut cut_of(const char* p, int n) {
+  using X = Ty<TY>;
+  const int to_line = (int)((128 - ((uintptr_t)p & 127)) & 127) / X::size;
+  const int head = min(n, to_line), nv = (n - head) / X::N;
+  return {head, nv, n - nv * X::N};
+}
+// where loose element i < loose lies, and where vector i begins
+template <int TY>
+DEVINL int loose_at(const Cut& cut, int i) {
+  return i < cut.head ? i : i + cut.nv * Ty<TY>::N;
+}
+
 // 2^a by the hardware instruction: results under 2^-126 are 0, which changes
 // no sum that has a term of 1 and no probability that a float can tell from 0.
 DEVINL float exp2_hw(float a) { return __builtin_amdgcn_exp2f(a); }
@@ -312,8 +333,9 @@ __global__ void __launch_bounds__(kThreads)
   const int v0 = sp * seg;
   const int n = min(seg, in.V - v0);
   const char* x = (const char*)in.x + (row_start(in, r) + v0) * X::size;
-  const float c = in.c;
-  const int nv = n / X::N;
+  const Cut cut = cut_of<TY>(x, n);
+  const int nv = cut.nv;
+  const char* xv = x + cut.head * X::size;
   const bool stay = (r & 15) < keep16;
   u32x4 first[Q];
 #pragma unroll
@@ -325,13 +347,13 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
     for (int g = 0; g < Q; ++g)
       if (tid + g * kThreads < nv)
-        first[g] = load16<false>(x + (long long)(tid + g * kThreads) * 16);
+        first[g] = load16<false>(xv + (long long)(tid + g * kThreads) * 16);
   } else {
     asm volatile("" ::: "memory");
 #pragma unroll
     for (int g = 0; g < Q; ++g)
       if (tid + g * kThreads < nv)
-        first[g] = load16<true>(x + (long long)(tid + g * kThreads) * 16);
+        first[g] = load16<true>(xv + (long long)(tid + g * kThreads) * 16);
   }
   if (xt && tid == 0) {
     const long long j = place(pl, r);
@@ -340,12 +362,20 @@ __global__ void __launch_bounds__(kThreads)
     else if (sp == 0 && (j < 0 || j >= in.V))
       xt[r] = NAN;  // a place outside the row
   }
+  const int loose_bits = (nv * X::N + 31) / 32 * 32;
   if (TOP) {
-    for (int i = tid; i < (n + 31) / 32; i += kThreads) bits[i] = 0;
+    // the vectors' elements from 0 on, the loose ones behind them
+    for (int i = tid; i < loose_bits / 32 + 3; i += kThreads) bits[i] = 0;
     __syncthreads();
     if (tid < pl.K) {
-      const long long j = place(pl, (long long)r * pl.K + tid) - v0;
-      if (j >= 0 && j < n) atomicOr(&bits[j >> 5], 1u << (j & 31));
+      const long long at = place(pl, (long long)r * pl.K + tid) - v0;
+      if (at >= 0 && at < n) {
+        const int j = (int)at;
+        const int b = j < cut.head                  ? loose_bits + j
+                      : j >= cut.head + nv * X::N ? loose_bits + j - nv * X::N
+                                                  : j - cut.head;
+        atomicOr(&bits[b >> 5], 1u << (b & 31));
+      }
     }
     __syncthreads();
   }
@@ -358,7 +388,7 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
       for (int g = 0; g < Q; ++g) {
         const int j = (i + g * kThreads) * X::N;
-        unsigned hit = j < n ? bits[j >> 5] >> (j & 31) : 0u;
+        unsigned hit = j < nv * X::N ? bits[j >> 5] >> (j & 31) : 0u;
         hit &= (1u << X::N) - 1u;
         if (hit) {
 #pragma unroll
@@ -386,7 +416,7 @@ __global__ void __launch_bounds__(kThreads)
       u32x4 raw[Q];
 #pragma unroll
       for (int g = 0; g < Q; ++g)
-        raw[g] = load16<nt.value>(x + (long long)(i + g * kThreads) * 16);
+        raw[g] = load16<nt.value>(xv + (long long)(i + g * kThreads) * 16);
       take(raw, i);
     }
     if (i < nv) {
@@ -395,7 +425,7 @@ __global__ void __launch_bounds__(kThreads)
       for (int g = 0; g < Q; ++g) {
         raw[g] = X::lowest();
         if (i + g * kThreads < nv)
-          raw[g] = load16<nt.value>(x + (long long)(i + g * kThreads) * 16);
+          raw[g] = load16<nt.value>(xv + (long long)(i + g * kThreads) * 16);
       }
       take(raw, i);
     }
@@ -404,10 +434,10 @@ __global__ void __launch_bounds__(kThreads)
     walk(std::false_type());
   else
     walk(std::true_type());
-  if (tid < n - nv * X::N) {  // what is left of a vector
-    int j = nv * X::N + tid;
-    float f = X::one(x + (long long)j * X::size);
-    if (TOP && (bits[j >> 5] >> (j & 31) & 1))
+  if (tid < cut.loose) {
+    const float f = X::one(x + loose_at<TY>(cut, tid) * X::size);
+    const int b = loose_bits + tid;
+    if (TOP && (bits[b >> 5] >> (b & 31) & 1))
       top.join(f, 1.f, in);
     else
       a.join(f, 1.f, in);
@@ -663,8 +693,10 @@ __global__ void __launch_bounds__(kThreads)
   const int r = in.R - 1 - row;
   const int v0 = sp * seg;
   const int n = min(seg, in.V - v0);
-  const int nv = n / X::N, left = n - nv * X::N;
   char* dx = dx_all + ((long long)r * in.V + v0) * X::size;
+  const Cut cut = cut_of<TY>(dx, n);
+  const int nv = cut.nv;
+  char* dxv = dx + cut.head * X::size;
   float a = kp.coef[r];
   if (a != 0.f) {
     if (up.per == LM_UP_ALL)
@@ -675,11 +707,12 @@ __global__ void __launch_bounds__(kThreads)
   if (a == 0.f) {
     const u32x4 zero = {0, 0, 0, 0};
     for (int i = tid; i < nv; i += kThreads)
-      store16<NT>(dx + (long long)i * 16, zero);
-    if (tid < left) X::put(dx + (long long)(nv * X::N + tid) * X::size, 0.f);
+      store16<NT>(dxv + (long long)i * 16, zero);
+    if (tid < cut.loose) X::put(dx + loose_at<TY>(cut, tid) * X::size, 0.f);
     return;
   }
   const char* x = (const char*)in.x + (row_start(in, r) + v0) * X::size;
+  const char* xv = x + cut.head * X::size;
   const LmStat st = kp.stat[r];
   const float c = in.c, mb = st.mb, w = a * st.w;
   const long long target = ONE ? place(pl, r) - v0 : -1;
@@ -702,34 +735,34 @@ __global__ void __launch_bounds__(kThreads)
       there = a * (st.mass_S * exp2_hw((xt - st.M) * c) - ps);
     }
   }
+  const long long aim = target - cut.head;
   auto put = [&](u32x4 raw, int ig) {
     float f[X::N];
     X::open(raw, f);
 #pragma unroll
     for (int e = 0; e < X::N; ++e) f[e] = w * exp2_hw((f[e] - mb) * c);
-    if (ONE && target >= (long long)ig * X::N &&
-        target < (long long)(ig + 1) * X::N) {
+    if (ONE && aim >= (long long)ig * X::N && aim < (long long)(ig + 1) * X::N) {
 #pragma unroll
       for (int e = 0; e < X::N; ++e)
-        if (target == (long long)ig * X::N + e) f[e] -= a;
+        if (aim == (long long)ig * X::N + e) f[e] -= a;
     }
-    store16<NT>(dx + (long long)ig * 16, X::close(f));
+    store16<NT>(dxv + (long long)ig * 16, X::close(f));
   };
   int i = tid;
   for (; i + (Q - 1) * kThreads < nv; i += Q * kThreads) {
     u32x4 raw[Q];
 #pragma unroll
     for (int g = 0; g < Q; ++g)
-      raw[g] = load16<true>(x + (long long)(i + g * kThreads) * 16);
+      raw[g] = load16<true>(xv + (long long)(i + g * kThreads) * 16);
 #pragma unroll
     for (int g = 0; g < Q; ++g) put(raw[g], i + g * kThreads);
   }
-  for (; i < nv; i += kThreads) put(load16<true>(x + (long long)i * 16), i);
-  if (tid < left) {
-    const int j = nv * X::N + tid;
-    float f = w * exp2_hw((X::one(x + (long long)j * X::size) - mb) * c);
+  for (; i < nv; i += kThreads) put(load16<true>(xv + (long long)i * 16), i);
+  if (tid < cut.loose) {
+    const int j = loose_at<TY>(cut, tid);
+    float f = w * exp2_hw((X::one(x + j * X::size) - mb) * c);
     if (ONE && target == j) f -= a;
-    X::put(dx + (long long)j * X::size, f);
+    X::put(dx + j * X::size, f);
   }
   if (!ONE) {
     __syncthreads();  // the row is written, now its places
@@ -756,7 +789,7 @@ DEVINL unsigned order_key(float f) {
   return f != f ? 0xffffffffu : order_of(f);  // above all, as in torch
 }
 
-constexpr int kCand = 2048;    // logits that reach the bound
+constexpr int kCand = 1984;    // logits that reach the bound; four blocks fit a CU
 constexpr int kPieces = 4096;  // maxima kept; piece i of a longer row is in i % kPieces
 
 // a logit that ranks, its place, and whether its zero was a negative one
@@ -790,7 +823,10 @@ __global__ void __launch_bounds__(THREADS)
   const int tid = threadIdx.x, r = blockIdx.x;
   const char* x = (const char*)in.x + row_start(in, r) * X::size;
   const float c = in.c;
-  const int V = in.V, nv = V / X::N, left = V - nv * X::N;
+  const int V = in.V;
+  const Cut cut = cut_of<TY>(x, V);
+  const int nv = cut.nv;
+  const char* xv = x + cut.head * X::size;
   if (tid == 0) n_share = n_cand = odd = 0;
   for (int i = tid; i < kPieces; i += THREADS) maxima[i] = -INFINITY;
   __syncthreads();
@@ -814,7 +850,7 @@ __global__ void __launch_bounds__(THREADS)
       if (PIECE == kLogits) {
         if (ig < nv) {
 #pragma unroll
-          for (int e = 0; e < X::N; ++e) maxima[ig * X::N + e] = f[g * X::N + e];
+          for (int e = 0; e < X::N; ++e) maxima[cut.head + ig * X::N + e] = f[g * X::N + e];
         }
         continue;
       }
@@ -838,7 +874,7 @@ __global__ void __launch_bounds__(THREADS)
     u32x4 raw[Q];
 #pragma unroll
     for (int g = 0; g < Q; ++g)
-      raw[g] = load16<NT>(x + (long long)(i + g * THREADS) * 16);
+      raw[g] = load16<NT>(xv + (long long)(i + g * THREADS) * 16);
     take(raw, i);
   }
   if ((i & ~63) < nv) {
@@ -847,13 +883,14 @@ __global__ void __launch_bounds__(THREADS)
     for (int g = 0; g < Q; ++g) {
       raw[g] = X::lowest();
       if (i + g * THREADS < nv)
-        raw[g] = load16<NT>(x + (long long)(i + g * THREADS) * 16);
+        raw[g] = load16<NT>(xv + (long long)(i + g * THREADS) * 16);
     }
     take(raw, i);
   }
-  if (tid < left) {
-    const float f = X::one(x + (long long)(nv * X::N + tid) * X::size);
-    if (PIECE == kLogits) maxima[nv * X::N + tid] = f;
+  if (tid < cut.loose) {
+    const int j = loose_at<TY>(cut, tid);
+    const float f = X::one(x + j * X::size);
+    if (PIECE == kLogits) maxima[j] = f;
     a.join(f, 1.f, in);
   }
   a = wave_join(a, in);
@@ -932,9 +969,9 @@ __global__ void __launch_bounds__(THREADS)
       else
         share[atomicAdd(&n_share, 1)] = (unsigned short)i;
     }
-  if (PIECE != kLogits && tid < left) {
-    const int j = nv * X::N + tid;
-    const float f = X::one(x + (long long)j * X::size);
+  if (PIECE != kLogits && tid < cut.loose) {
+    const int j = loose_at<TY>(cut, tid);
+    const float f = X::one(x + j * X::size);
     if (f >= bound) offer(f, j);
   }
   __syncthreads();
@@ -945,7 +982,7 @@ __global__ void __launch_bounds__(THREADS)
         const int ig = ((from + share[i >> SHIFT]) << SHIFT) + (i & ((1 << SHIFT) - 1));
         if (ig >= nv) continue;
         float f[X::N];
-        X::open(*(const u32x4_any*)(x + (long long)ig * 16), f);
+        X::open(load16<false>(xv + (long long)ig * 16), f);
         int hits = 0;
 #pragma unroll
         for (int e = 0; e < X::N; ++e) hits += f[e] >= bound;
@@ -954,7 +991,7 @@ __global__ void __launch_bounds__(THREADS)
 #pragma unroll
         for (int e = 0; e < X::N; ++e)
           if (f[e] >= bound) {
-            if (at < kCand) cand[at] = candidate(f[e], ig * X::N + e);
+            if (at < kCand) cand[at] = candidate(f[e], cut.head + ig * X::N + e);
             ++at;
           }
       }
@@ -967,13 +1004,13 @@ __global__ void __launch_bounds__(THREADS)
     auto each = [&](auto&& use) {
       for (int i = tid; i < nv; i += THREADS) {
         float f[X::N];
-        X::open(load16<false>(x + (long long)i * 16), f);
+        X::open(load16<false>(xv + (long long)i * 16), f);
 #pragma unroll
-        for (int e = 0; e < X::N; ++e) use(candidate(f[e], i * X::N + e));
+        for (int e = 0; e < X::N; ++e) use(candidate(f[e], cut.head + i * X::N + e));
       }
-      if (tid < left) {
-        const int j = nv * X::N + tid;
-        use(candidate(X::one(x + (long long)j * X::size), j));
+      if (tid < cut.loose) {
+        const int j = loose_at<TY>(cut, tid);
+        use(candidate(X::one(x + j * X::size), j));
       }
     };
     unsigned long long t = 0;
@@ -1050,9 +1087,11 @@ long long bytes_of(const LmRows& in) {
 
 constexpr int kStatBlocks = 1024, kStatSeg = 131072;
 constexpr int kGradBlocks = 2048, kGradSeg = 32768;
-// At 1024 rows of 128256 blocks of 1024 threads take as long (56 us) and those
-// of 256 longer (64); at 4000 rows of 8000 512 take 44 us, 1024 take 72.
-constexpr int kTopkThreads = 512;
+// Threads of a block of topk: 512, or 1024 where there are no more rows than
+// CUs and each is long. At 1024 rows of 128256 both take 56 us (256 threads
+// 64), at 4000 rows of 8000 512 take 44 us and 1024 take 72, at 100 rows of
+// 262144 33 and 27.
+constexpr int kTopkFewRows = 256, kTopkLongRow = 8192;  // vectors
 
 // What the pass over a row leaves in the 256 MB cache behind the L2, the pass
 // of the gradient need not fetch again. At 525 MB of logits a cache that every
@@ -1092,24 +1131,32 @@ void stats_of(const LmRows& in, const LmPlaces& pl, const LmTeacher& te,
   auto kernel = top         ? lm_stats_kernel<TY, true, true>
                 : te.values ? lm_stats_kernel<TY, true, false>
                             : lm_stats_kernel<TY, false, false>;
-  kernel<<<grid, kThreads, top ? (seg + 31) / 32 * 4 : 0, s>>>(
+  kernel<<<grid, kThreads, top ? ((seg + 31) / 32 + 3) * 4 : 0, s>>>(
       in, pl, te, splits, seg, keep16, w.part, w.part_top, w.xt, kp.p, w.rec,
       w.counter);
+}
+
+template <int TY, int T, int PIECE>
+void topk_with(const LmRows& in, float temperature, int k, void* values,
+               long long* indices, float* lse, hipStream_t s) {
+  auto kernel = bytes_of(in) > kStreamTopk ? lm_topk_kernel<TY, T, PIECE, true>
+                                           : lm_topk_kernel<TY, T, PIECE, false>;
+  kernel<<<dim3(in.R), T, 0, s>>>(in, temperature, k, (char*)values, indices, lse);
 }
 
 template <int TY>
 void topk_of(const LmRows& in, float temperature, int k, void* values,
              long long* indices, float* lse, hipStream_t s) {
-  constexpr int T = kTopkThreads;
-  const bool nt = bytes_of(in) > kStreamTopk;
   const int nv = in.V / Ty<TY>::N;
   // lines where there are four of them and more to each of the k
-  const int piece = in.V <= kPieces ? kLogits : nv >= 32 * k ? kLines : kVectors;
-  auto kernel =
-      piece == kLogits  ? (nt ? lm_topk_kernel<TY, T, kLogits, true> : lm_topk_kernel<TY, T, kLogits, false>)
-      : piece == kLines ? (nt ? lm_topk_kernel<TY, T, kLines, true> : lm_topk_kernel<TY, T, kLines, false>)
-                        : (nt ? lm_topk_kernel<TY, T, kVectors, true> : lm_topk_kernel<TY, T, kVectors, false>);
-  kernel<<<dim3(in.R), T, 0, s>>>(in, temperature, k, (char*)values, indices, lse);
+  if (in.V <= kPieces)
+    topk_with<TY, 512, kLogits>(in, temperature, k, values, indices, lse, s);
+  else if (nv < 32 * k)
+    topk_with<TY, 512, kVectors>(in, temperature, k, values, indices, lse, s);
+  else if (in.R <= kTopkFewRows && nv > kTopkLongRow)
+    topk_with<TY, 1024, kLines>(in, temperature, k, values, indices, lse, s);
+  else
+    topk_with<TY, 512, kLines>(in, temperature, k, values, indices, lse, s);
 }
 
 #define LM_BY_TYPE(type, call)            \

@@ -16,8 +16,8 @@ _KERNEL_TYPES = (torch.bfloat16, torch.float16, torch.float32)
 
 
 def check_logits(logits: torch.Tensor) -> None:
-    if logits.dim() < 1 or logits.shape[-1] < 1:
-        raise ValueError("logits must be [..., V] with V >= 1")
+    if logits.dim() < 1 or not 1 <= logits.shape[-1] < 1 << 28:
+        raise ValueError("logits must be [..., V] with 1 <= V < 2**28")
     if logits.dtype not in _KERNEL_TYPES and (
             logits.is_cuda or logits.dtype != torch.float64):
         raise ValueError("logits must be bfloat16, float16 or float32 "
