@@ -706,7 +706,8 @@ def test_refusals(device):
         lambda: policy_loss(x, targets, rows, rows, mask=targets),
     ]
     if device == "cuda":
-        bad += [lambda: topk_logits(x.double(), 2),
+        bad += [lambda: topk_logits(x[0, 0, :1].expand(1 << 22, 1), 1),
+                lambda: topk_logits(x.double(), 2),
                 lambda: policy_loss(x, targets.cpu(), rows, rows),
                 lambda: preference_loss(x, targets, ref.cpu()),
                 lambda: distill_loss(x, values.cpu(), indices)]
@@ -765,6 +766,50 @@ def test_gradient_reaches_views_and_accumulates():
     _, _, grad, _, _ = preference_oracle(base[:, :-1, :512], targets, ref, 0.1, 0.0, -100)
     assert (base.grad[:, -1] == 0).all() and (base.grad[..., 512:] == 0).all()
     torch.testing.assert_close(base.grad[:, :-1, :512].cpu().double(), grad, rtol=1e-3, atol=1e-6)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_rows_of_several_segments(dtype):
+    """A vocabulary that no single block takes, beside many short rows."""
+    need("cuda")
+    scale = 512.0 if dtype == torch.float16 else 1.0
+    for B, T, V in ((1, 2, 300001), (6, 301, 97)):
+        x = make_logits(B, T, V, dtype, "cuda")
+        up = torch.tensor(scale, device="cuda")
+        values, indices, lse = make_record(x, 40, 2.0)
+        check_distill(x, values, indices, lse, 2.0, up=up)
+        check_distill(x, values, indices, None, 2.0, up=up)
+        check_policy(x, *make_rollout(x), up=up)
+        check_preference(x.repeat(2, 1, 1), *make_pairs(B, T, V, "cuda"), up=up)
+
+
+@pytest.mark.gpu
+def test_no_grad_and_inference_mode():
+    need("cuda")
+    x = make_logits(4, 9, 515, torch.bfloat16, "cuda").requires_grad_(True)
+    values, indices, lse = make_record(x, 5, 2.0)
+    args = make_pairs(2, 9, 515, "cuda"), make_rollout(x), (values, indices), lse
+    want = [l.item() for l in all_losses(x, *args)]
+    for mode in (torch.no_grad, torch.inference_mode):
+        with mode():
+            got = all_losses(x, *args)
+            assert not any(l.requires_grad for l in got)
+            assert [l.item() for l in got] == want
+            assert topk_logits(x.clone(), 3).values.shape == (4, 9, 3)
+
+
+@pytest.mark.gpu
+def test_changed_logits_are_noticed():
+    """The gradient is made from the logits that the loss saw, or not at all."""
+    need("cuda")
+    x = make_logits(1, 3, 64, torch.float32, "cuda").requires_grad_(True)
+    values, indices, _ = make_record(x, 4, 1.0)
+    y = x * 1.0
+    loss = distill_loss(y, values, indices)
+    y.mul_(2.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
 
 
 @pytest.mark.gpu

@@ -4,7 +4,7 @@ Argument checks, the layout that the kernels read, and the row softmax of
 the CPU path. The kernels take ``[V]``, ``[T, V]`` or ``[B, T, V]`` logits
 whose rows may lie anywhere (a slice ``logits[:, :-1]`` is read in place);
 more dimensions are folded into ``B``, and logits whose last dimension is
-not contiguous are copied once.
+not contiguous are copied once. A call takes up to 2**22 - 1 rows.
 """
 from __future__ import annotations
 
@@ -18,6 +18,8 @@ _KERNEL_TYPES = (torch.bfloat16, torch.float16, torch.float32)
 def check_logits(logits: torch.Tensor) -> None:
     if logits.dim() < 1 or not 1 <= logits.shape[-1] < 1 << 28:
         raise ValueError("logits must be [..., V] with 1 <= V < 2**28")
+    if logits.is_cuda and logits.numel() >= logits.shape[-1] << 22:
+        raise ValueError("logits must be of fewer than 2**22 rows a call")
     if logits.dtype not in _KERNEL_TYPES and (
             logits.is_cuda or logits.dtype != torch.float64):
         raise ValueError("logits must be bfloat16, float16 or float32 "
