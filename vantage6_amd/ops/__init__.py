@@ -10,6 +10,8 @@ north star):
 - ``optim``     — fused SGD-momentum / AdamW on flat parameter buffers
 - ``dp``        — DP-SGD per-sample clip + Philox gaussian noise
 - ``secagg``    — pairwise Philox secure-aggregation masks
+- ``distill``   — records of top logits, and the divergence from them
+- ``preference`` — paired log-ratio loss, clipped policy loss with a KL term
 
 Dispatch policy: on CUDA(HIP) tensors the hand-written extension is
 REQUIRED — a missing extension raises instead of silently falling back to
