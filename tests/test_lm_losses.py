@@ -341,7 +341,7 @@ def preference_oracle(logits, targets, ref, beta, eps, ignore):
     r = beta * (lp.sum(-1) - ref.cpu().double())
     z = r[:N] - r[N:]
     loss = -((1 - eps) * torch.nn.functional.logsigmoid(z) + eps * torch.nn.functional.logsigmoid(-z))
-    by_z = torch.sigmoid(z) - (1 - eps)
+    by_z = eps - torch.sigmoid(-z)  # sigmoid(z) - (1 - eps)
     a = beta * torch.cat([by_z, -by_z])[:, None] * keep
     one = torch.zeros_like(lq).scatter_(-1, tg.clamp_min(0)[..., None], 1.0)
     grad = torch.where(a[..., None] != 0, a[..., None] * (one - lq.exp()), 0.0)
@@ -433,6 +433,19 @@ def test_preference_far_margins(device):
     targets = torch.zeros(4, 3, dtype=torch.int64, device=device)
     ref = torch.tensor([-1e6, 1e6, 0.0, 0.0], device=device)
     check_preference(x, targets, ref, reduction="none")
+    # z = 40 and -40: a pair that is all but settled has a gradient of e^-40
+    lp = softmax64(x)[..., 0].sum(-1)
+    ref = lp - torch.tensor([400.0, -400.0, 0.0, 0.0], dtype=torch.float64)
+    y = x.clone().requires_grad_(True)
+    out = preference_loss(y, targets, ref.to(device), reduction="none")
+    grad, = torch.autograd.grad(out.loss.sum(), y)
+    want = [0.1 * math.exp(-40.0), 0.1]
+    for pair in range(2):
+        for row in (pair, pair + 2):
+            a = grad[row, 0, 0].item() / (softmax64(x)[row, 0, 0].exp().item() - 1)
+            a = a if row < 2 else -a
+            # z is off by 6 LP of its rewards
+            assert abs(a / want[pair] - 1) < 6 * LP + GRAD, (row, a)
 
 
 @pytest.mark.parametrize("device", CPU_GPU)

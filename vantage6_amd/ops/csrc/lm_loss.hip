@@ -646,7 +646,7 @@ __global__ void __launch_bounds__(1024)
     }
   }
   block_sum2(sum[0], sum[1], red);
-  double loss = 0.0;
+  double loss = 0.0, z = 0.0, low = 0.0;
   if (threadIdx.x == 0) {
     double reward[2];
 #pragma unroll
@@ -656,17 +656,22 @@ __global__ void __launch_bounds__(1024)
                                   : (double)((const float*)pr.ref)[b];
       reward[side] = pr.beta * (sum[side] - ref);
     }
-    // -log sigmoid(z) = max(-z, 0) + log(1 + exp(-|z|))
-    const double z = reward[0] - reward[1], e = pr.smoothing;
-    const double both = log1p(exp(-fabs(z)));
-    loss = (1.0 - e) * (fmax(-z, 0.0) + both);
-    if (e != 0.0) loss += e * (fmax(z, 0.0) + both);
-    s_a = (float)(pr.beta * (1.0 - e - 1.0 / (1.0 + exp(-z))));
+    z = reward[0] - reward[1];
+    low = exp(-fabs(z));
+    // 1 - sigmoid(z), without the difference
+    const double away = (z < 0.0 ? 1.0 : low) / (1.0 + low);
+    s_a = (float)(pr.beta * (away - pr.smoothing));
     chosen[n] = (float)reward[0];
     rejected[n] = (float)reward[1];
-    if (o.reduction == LM_NONE) o.loss[n] = (float)loss;
   }
   __syncthreads();
+  if (threadIdx.x == 0) {
+    // -log sigmoid(z) = max(-z, 0) + log(1 + exp(-|z|))
+    const double e = pr.smoothing, both = log1p(low);
+    loss = (1.0 - e) * (fmax(-z, 0.0) + both);
+    if (e != 0.0) loss += e * (fmax(z, 0.0) + both);
+    if (o.reduction == LM_NONE) o.loss[n] = (float)loss;
+  }
   // the gradient is coef * (q - onehot), and the other way for the rejected
   const float a = s_a;
   for (int t = threadIdx.x; t < 2 * T; t += blockDim.x) {
