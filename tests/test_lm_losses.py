@@ -856,6 +856,36 @@ def test_another_stream():
 
 
 @pytest.mark.gpu
+def test_two_streams_at_once():
+    """Calls that overlap on two streams share nothing."""
+    need("cuda")
+    sides, want, got = [torch.cuda.Stream() for _ in range(2)], [], [[], []]
+    sets = []
+    for seed in (0, 1):
+        x = make_logits(4, 64, 30522, torch.bfloat16, "cuda", seed=seed).requires_grad_(True)
+        values, indices, lse = make_record(x, 9, 2.0, seed=seed)
+        sets.append((x, make_pairs(2, 64, 30522, "cuda", seed=seed), make_rollout(x, seed=seed),
+                     (values, indices), lse))
+
+    def step(args):
+        losses = all_losses(*args)
+        grads = [torch.autograd.grad(l, args[0])[0] for l in losses]
+        return [l.detach() for l in losses] + grads + list(topk_logits(args[0], 5))
+
+    for args in sets:
+        want.append(step(args))
+    torch.cuda.synchronize()
+    for _ in range(4):
+        for i, side in enumerate(sides):
+            with torch.cuda.stream(side):
+                got[i].append(step(sets[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for out in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(out, want[i]))
+
+
+@pytest.mark.gpu
 def test_two_captured_graphs():
     """Forward and backward in two graphs that share nothing, replayed in turn
     on new inputs with eager calls between."""

@@ -584,9 +584,9 @@ static LmRows lm_rows(const torch::Tensor& x, double temperature) {
   in.V = (int)V;
   in.type = lm_type(x, "logits");
   const double c = 1.4426950408889634074 / temperature;
-  in.c = (float)c;
-  if ((double)in.c >= c) in.c = std::nextafterf(in.c, 0.f);
-  in.c_lo = (float)(c - in.c);  // > 0
+  in.c = in.c_hi = (float)c;
+  if ((double)in.c_hi >= c) in.c_hi = std::nextafterf(in.c_hi, 0.f);
+  in.c_lo = (float)(c - in.c_hi);
   return in;
 }
 
@@ -673,7 +673,7 @@ std::vector<torch::Tensor> lm_topk_fwd(torch::Tensor x, int64_t k,
   sizes.pop_back();
   auto lse = torch::empty(sizes, opt.dtype(torch::kFloat32));
   if (in.R)
-    lm_topk(in, (float)temperature, (int)k, values.data_ptr(),
+    lm_topk(in, temperature, (int)k, values.data_ptr(),
             (long long*)idx.data_ptr(), lse.data_ptr<float>(), cur_stream());
   return {values, idx, lse};
 }
@@ -732,7 +732,7 @@ struct LmDistillFn : public torch::autograd::Function<LmDistillFn> {
     pl.mask = (const uint8_t*)lm_ptr(mask);
     pl.K = (int)K;
     LmTeacher te{values.data_ptr(), (const float*)lm_ptr(lse),
-                 lm_type(values, "teacher_values"), (float)temperature};
+                 lm_type(values, "teacher_values"), temperature};
     LmKeep kp;
     LmWork w;
     auto keep = lm_keep(x, in, pl.K, lse.has_value(), 0, &kp, &w);

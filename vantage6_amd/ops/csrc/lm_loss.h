@@ -13,7 +13,8 @@ struct LmRows {
   long long sb, st;
   int T, R, V;
   int type;
-  float c, c_lo;  // log2(e) / temperature, and what a float leaves of it
+  float c;           // log2(e) / temperature
+  float c_hi, c_lo;  // the same in two parts, both positive
 };
 
 // What the backward pass keeps of a row: base gradient coef * w * 2^((x-mb)c),
@@ -67,7 +68,7 @@ struct LmTeacher {
   const void* values;  // [R, K] of `type`
   const float* lse;    // [R], or null: the record is renormalised
   int type;
-  float temperature;
+  double temperature;
 };
 
 struct LmPolicy {
@@ -100,5 +101,5 @@ void lm_preference(const LmRows& in, const LmPlaces& pl, const LmPreference& pr,
 // dx: [R, V], side by side
 void lm_grad(const LmRows& in, const LmPlaces& pl, const LmKeep& kp,
              const LmUp& up, void* dx, hipStream_t s);
-void lm_topk(const LmRows& in, float temperature, int k, void* values,
+void lm_topk(const LmRows& in, double temperature, int k, void* values,
              long long* indices, float* lse, hipStream_t s);

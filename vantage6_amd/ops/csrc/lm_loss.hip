@@ -153,10 +153,10 @@ DEVINL float exp2_hw(float a) { return __builtin_amdgcn_exp2f(a); }
 
 // 2^(d log2(e)/t) with the constant in two parts: one float of it is off by up
 // to 2^-25, the same way for every logit, and that would be 1e-7 in log S, in
-// one direction for all the tokens of an answer. The second part is positive,
-// so that a d of -inf stays one.
+// one direction for all the tokens of an answer. Both parts are positive, so
+// that a d of -inf stays one.
 DEVINL float exp_of(float d, const LmRows& in) {
-  return exp2_hw(fmaf(d, in.c, d * in.c_lo));
+  return exp2_hw(fmaf(d, in.c_hi, d * in.c_lo));
 }
 
 // Reductions over a wave by DPP moves, a few cycles each where a shuffle
@@ -814,7 +814,7 @@ DEVINL float logit_of(unsigned long long cand) {
 
 template <int TY, int THREADS, int PIECE, bool NT>
 __global__ void __launch_bounds__(THREADS)
-    lm_topk_kernel(LmRows in, float temperature, int k,
+    lm_topk_kernel(LmRows in, double temperature, int k,
                    char* __restrict__ values,
                    long long* __restrict__ indices, float* __restrict__ lse) {
   using X = Ty<TY>;
@@ -1142,7 +1142,7 @@ void stats_of(const LmRows& in, const LmPlaces& pl, const LmTeacher& te,
 }
 
 template <int TY, int T, int PIECE>
-void topk_with(const LmRows& in, float temperature, int k, void* values,
+void topk_with(const LmRows& in, double temperature, int k, void* values,
                long long* indices, float* lse, hipStream_t s) {
   auto kernel = bytes_of(in) > kStreamTopk ? lm_topk_kernel<TY, T, PIECE, true>
                                            : lm_topk_kernel<TY, T, PIECE, false>;
@@ -1150,7 +1150,7 @@ void topk_with(const LmRows& in, float temperature, int k, void* values,
 }
 
 template <int TY>
-void topk_of(const LmRows& in, float temperature, int k, void* values,
+void topk_of(const LmRows& in, double temperature, int k, void* values,
              long long* indices, float* lse, hipStream_t s) {
   const int nv = in.V / Ty<TY>::N;
   // lines where there are four of them and more to each of the k
@@ -1247,7 +1247,7 @@ void lm_grad(const LmRows& in, const LmPlaces& pl, const LmKeep& kp,
   LM_BY_TYPE(in.type, (grad_of<TY>(in, pl, kp, up, dx, s)));
 }
 
-void lm_topk(const LmRows& in, float temperature, int k, void* values,
+void lm_topk(const LmRows& in, double temperature, int k, void* values,
              long long* indices, float* lse, hipStream_t s) {
   LM_BY_TYPE(in.type, (topk_of<TY>(in, temperature, k, values, indices, lse, s)));
 }
