@@ -1090,8 +1090,14 @@ long long bytes_of(const LmRows& in) {
   return (long long)in.R * in.V * (in.type == LM_FP32 ? 4 : 2);
 }
 
-constexpr int kStatBlocks = 1024, kStatSeg = 131072;
-constexpr int kGradBlocks = 2048, kGradSeg = 32768;
+// Blocks that a pass asks for at least, splitting rows: of stats 512 (64 rows of
+// 30522: 4.5 us, with 1024 5.8; 200 of 128256 14, with 256 too), of grad 2048
+// (700 rows of 30522 16 us, with 512 18).
+constexpr int kStatBlocks = 512, kGradBlocks = 2048;
+// A segment's most: of stats what its bits in LDS allow; of grad four rounds of
+// loads a thread while the cache holds the logits (4096 rows of 30522 fp16 72
+// us, in one round 75), else one (2048 rows of 128256 151 us, in four 159).
+constexpr int kStatSeg = 131072, kGradSegBytes = 65536, kGradSegFar = 16384;
 // Threads of a block of topk: 512, or 1024 where there are no more rows than
 // CUs and each is long. At 1024 rows of 128256 both take 56 us (256 threads
 // 64), at 4000 rows of 8000 512 take 44 us and 1024 take 72, at 100 rows of
@@ -1112,11 +1118,16 @@ constexpr long long kStreamGrad = 64 * kMB;
 // 60 us, at 78 MB 22 against 20.
 constexpr long long kStreamTopk = 128 * kMB;
 
+int grad_seg(const LmRows& in) {
+  return (bytes_of(in) > kKeepBytes ? kGradSegFar : kGradSegBytes) /
+         (in.type == LM_FP32 ? 4 : 2);
+}
+
 template <int TY>
 void grad_of(const LmRows& in, const LmPlaces& pl, const LmKeep& kp,
              const LmUp& up, void* dx, hipStream_t s) {
   int seg;
-  const int splits = splits_for(in, kGradBlocks, kGradSeg, &seg);
+  const int splits = splits_for(in, kGradBlocks, grad_seg(in), &seg);
   const dim3 grid((unsigned)in.R * splits);
   const bool nt = bytes_of(in) > kStreamGrad;
   auto kernel = kp.p ? (nt ? lm_grad_kernel<TY, false, true> : lm_grad_kernel<TY, false, false>)
@@ -1192,7 +1203,7 @@ int lm_stats_splits(const LmRows& in) {
 
 int lm_grad_splits(const LmRows& in) {
   int seg;
-  return splits_for(in, kGradBlocks, kGradSeg, &seg);
+  return splits_for(in, kGradBlocks, grad_seg(in), &seg);
 }
 
 int lm_group(int splits) {
@@ -1203,11 +1214,11 @@ int lm_group(int splits) {
 
 // The finish kernels are a chain of latencies: one block where it holds all the
 // rows, so that no block waits for another, else blocks of a wave while they
-// are a few hundred.
+// are few (2048 rows: 6.5 us, in blocks of 256 7.4; 16384 rows 10.6 and 7.4).
 static int finish_threads(int R, int group) {
   const long long lanes = (long long)R * group;
   if (lanes <= kThreads) return std::max(64, (int)(lanes + 63) / 64 * 64);
-  return lanes <= 16384 ? 64 : kThreads;
+  return lanes <= 8192 ? 64 : kThreads;
 }
 
 int lm_finish_blocks(int R, int group) {
