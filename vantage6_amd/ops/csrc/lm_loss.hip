@@ -305,8 +305,8 @@ DEVINL void record_of(const LmRows& in, const LmPlaces& pl, const LmTeacher& te,
 // kept apart: a bit per logit of the segment in LDS, so that the sum outside
 // the record is one of its own and not the difference of two that nearly
 // cancel.
-template <int TY, bool REC, bool TOP>
-__global__ void __launch_bounds__(kThreads)
+template <int TY, int THREADS, bool REC, bool TOP>
+__global__ void __launch_bounds__(THREADS)
     lm_stats_kernel(LmRows in, LmPlaces pl, LmTeacher te, int splits, int seg,
                     int keep16, float2* __restrict__ part,
                     float2* __restrict__ part_top, float* __restrict__ xt,
@@ -314,12 +314,12 @@ __global__ void __launch_bounds__(kThreads)
                     int* __restrict__ counter) {
   using X = Ty<TY>;
   extern __shared__ unsigned bits[];
-  __shared__ Run red[kThreads / 64];
+  __shared__ Run red[THREADS / 64];
   const int tid = threadIdx.x;
   if (blockIdx.x == 0 && tid == 0) *counter = 0;  // for the finish kernel
   int block = blockIdx.x;
   if (REC) {
-    constexpr int W = kThreads / 64;
+    constexpr int W = THREADS / 64;
     const int records = (in.R + W - 1) / W;
     if (block < records) {
       const int r = block * W + (tid >> 6);
@@ -346,14 +346,14 @@ __global__ void __launch_bounds__(kThreads)
     asm volatile("" ::: "memory");
 #pragma unroll
     for (int g = 0; g < Q; ++g)
-      if (tid + g * kThreads < nv)
-        first[g] = load16<false>(xv + (long long)(tid + g * kThreads) * 16);
+      if (tid + g * THREADS < nv)
+        first[g] = load16<false>(xv + (long long)(tid + g * THREADS) * 16);
   } else {
     asm volatile("" ::: "memory");
 #pragma unroll
     for (int g = 0; g < Q; ++g)
-      if (tid + g * kThreads < nv)
-        first[g] = load16<true>(xv + (long long)(tid + g * kThreads) * 16);
+      if (tid + g * THREADS < nv)
+        first[g] = load16<true>(xv + (long long)(tid + g * THREADS) * 16);
   }
   if (xt && tid == 0) {
     const long long j = place(pl, r);
@@ -365,10 +365,10 @@ __global__ void __launch_bounds__(kThreads)
   const int loose_bits = (nv * X::N + 31) / 32 * 32;
   if (TOP) {
     // the vectors' elements from 0 on, the loose ones behind them
-    for (int i = tid; i < loose_bits / 32 + 3; i += kThreads) bits[i] = 0;
+    for (int i = tid; i < loose_bits / 32 + 3; i += THREADS) bits[i] = 0;
     __syncthreads();
-    if (tid < pl.K) {
-      const long long at = place(pl, (long long)r * pl.K + tid) - v0;
+    for (int k = tid; k < pl.K; k += THREADS) {
+      const long long at = place(pl, (long long)r * pl.K + k) - v0;
       if (at >= 0 && at < n) {
         const int j = (int)at;
         const int b = j < cut.head                  ? loose_bits + j
@@ -387,7 +387,7 @@ __global__ void __launch_bounds__(kThreads)
     if (TOP) {
 #pragma unroll
       for (int g = 0; g < Q; ++g) {
-        const int j = (i + g * kThreads) * X::N;
+        const int j = (i + g * THREADS) * X::N;
         unsigned hit = j < nv * X::N ? bits[j >> 5] >> (j & 31) : 0u;
         hit &= (1u << X::N) - 1u;
         if (hit) {
@@ -411,12 +411,12 @@ __global__ void __launch_bounds__(kThreads)
   };
   take(first, tid);
   auto walk = [&](auto nt) {
-    int i = tid + Q * kThreads;
-    for (; i + (Q - 1) * kThreads < nv; i += Q * kThreads) {
+    int i = tid + Q * THREADS;
+    for (; i + (Q - 1) * THREADS < nv; i += Q * THREADS) {
       u32x4 raw[Q];
 #pragma unroll
       for (int g = 0; g < Q; ++g)
-        raw[g] = load16<nt.value>(xv + (long long)(i + g * kThreads) * 16);
+        raw[g] = load16<nt.value>(xv + (long long)(i + g * THREADS) * 16);
       take(raw, i);
     }
     if (i < nv) {
@@ -424,8 +424,8 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
       for (int g = 0; g < Q; ++g) {
         raw[g] = X::lowest();
-        if (i + g * kThreads < nv)
-          raw[g] = load16<nt.value>(xv + (long long)(i + g * kThreads) * 16);
+        if (i + g * THREADS < nv)
+          raw[g] = load16<nt.value>(xv + (long long)(i + g * THREADS) * 16);
       }
       take(raw, i);
     }
@@ -434,18 +434,18 @@ __global__ void __launch_bounds__(kThreads)
     walk(std::false_type());
   else
     walk(std::true_type());
-  if (tid < cut.loose) {
-    const float f = X::one(x + loose_at<TY>(cut, tid) * X::size);
-    const int b = loose_bits + tid;
+  for (int i = tid; i < cut.loose; i += THREADS) {
+    const float f = X::one(x + loose_at<TY>(cut, i) * X::size);
+    const int b = loose_bits + i;
     if (TOP && (bits[b >> 5] >> (b & 31) & 1))
       top.join(f, 1.f, in);
     else
       a.join(f, 1.f, in);
   }
-  a = block_join<kThreads>(a, in, red);
+  a = block_join<THREADS>(a, in, red);
   if (TOP) {
     __syncthreads();
-    top = block_join<kThreads>(top, in, red);
+    top = block_join<THREADS>(top, in, red);
   }
   if (tid == 0) {
     const long long at = (long long)r * splits + sp;
@@ -1135,21 +1135,37 @@ void grad_of(const LmRows& in, const LmPlaces& pl, const LmKeep& kp,
   kernel<<<grid, kThreads, 0, s>>>(in, pl, kp, up, (char*)dx, splits, seg);
 }
 
+// Many short rows take a wave each: a block's start, its joins through LDS and
+// its end outweigh such a row. 8192 rows of 600 bf16 8 us, in blocks of 256
+// threads 23; 60000 of 5001 112 and 157; 4096 of 16000 24 and 25. A wave alone is
+// behind with few rows (512 of 5001 fp32 5.2 and 4.4 us, 1024 of 8200 8.8 and
+// 6.8) and with longer ones (8192 of 30522 bf16 with a record 86 and 82).
+constexpr int kWaveRows = 2048, kWaveVectors = 2048;
+
+template <int TY, int T>
+void stats_with(const LmRows& in, const LmPlaces& pl, const LmTeacher& te,
+                const LmWork& w, const LmKeep& kp, int splits, int seg,
+                hipStream_t s) {
+  const dim3 grid((unsigned)in.R * splits + (te.values ? div_up(in.R, T / 64) : 0));
+  const int keep16 = (int)std::min(16LL, 16 * kKeepBytes / bytes_of(in));
+  const bool top = w.part_top != nullptr;
+  auto kernel = top         ? lm_stats_kernel<TY, T, true, true>
+                : te.values ? lm_stats_kernel<TY, T, true, false>
+                            : lm_stats_kernel<TY, T, false, false>;
+  kernel<<<grid, T, top ? ((seg + 31) / 32 + 3) * 4 : 0, s>>>(
+      in, pl, te, splits, seg, keep16, w.part, w.part_top, w.xt, kp.p, w.rec,
+      w.counter);
+}
+
 template <int TY>
 void stats_of(const LmRows& in, const LmPlaces& pl, const LmTeacher& te,
               const LmWork& w, const LmKeep& kp, hipStream_t s) {
   int seg;
   const int splits = splits_for(in, kStatBlocks, kStatSeg, &seg);
-  const dim3 grid((unsigned)in.R * splits +
-                  (te.values ? div_up(in.R, kThreads / 64) : 0));
-  const int keep16 = (int)std::min(16LL, 16 * kKeepBytes / bytes_of(in));
-  const bool top = w.part_top != nullptr;
-  auto kernel = top         ? lm_stats_kernel<TY, true, true>
-                : te.values ? lm_stats_kernel<TY, true, false>
-                            : lm_stats_kernel<TY, false, false>;
-  kernel<<<grid, kThreads, top ? ((seg + 31) / 32 + 3) * 4 : 0, s>>>(
-      in, pl, te, splits, seg, keep16, w.part, w.part_top, w.xt, kp.p, w.rec,
-      w.counter);
+  if (in.R >= kWaveRows && in.V / Ty<TY>::N <= kWaveVectors)
+    stats_with<TY, 64>(in, pl, te, w, kp, splits, seg, s);
+  else
+    stats_with<TY, kThreads>(in, pl, te, w, kp, splits, seg, s);
 }
 
 template <int TY, int T, int PIECE>
