@@ -1057,6 +1057,22 @@ def test_objectives_of_the_models(device, name, objective):
 
 
 @pytest.mark.parametrize("device", CPU_GPU)
+def test_preference_objective_with_another_ignore_index(device):
+    """What the mask leaves out stays out under any ``ignore_index``."""
+    need(device)
+    from vantage6_amd.models import build_model, model_loss
+
+    torch.manual_seed(2)
+    name, vocab = "llama_1b", TINY["llama_1b"]["vocab"]
+    model = build_model(name, device=device, **TINY[name])
+    batch = {k: v.to(device) for k, v in objective_data(model, vocab, "preference").items()}
+    with torch.no_grad():
+        want, got = (model_loss(name, "preference", **o)(model, batch)
+                     for o in ({}, {"ignore_index": -1}))
+    assert torch.isfinite(want) and torch.equal(got, want)
+
+
+@pytest.mark.parametrize("device", CPU_GPU)
 @pytest.mark.parametrize("objective", list(OPTIONS))
 def test_fit_rounds_with_an_objective(device, objective):
     need(device)

@@ -66,6 +66,8 @@ def _distill_objective(options) -> Callable:
 def _preference_objective(options) -> Callable:
     """Batch: ``input_ids`` [N, 2, S] (chosen, rejected), ``ref_logps`` [N, 2],
     optionally ``mask`` [N, 2, S], True where a token is one of the answer."""
+    ignore = options.get("ignore_index", -100)
+
     def loss(model, batch):
         from ..ops.preference import preference_loss
 
@@ -73,7 +75,7 @@ def _preference_objective(options) -> Callable:
         targets = ids[:, 1:]
         if "mask" in batch:
             mask = batch["mask"].transpose(0, 1).flatten(0, 1)[:, 1:]
-            targets = torch.where(mask, targets, -100)
+            targets = torch.where(mask, targets, ignore)
         ref = batch["ref_logps"].transpose(0, 1).flatten()
         return preference_loss(_lm_logits(model, ids[:, :-1]), targets, ref,
                                **options).loss
