@@ -331,6 +331,24 @@ def test_distill_index_outside_is_nan(device):
     assert torch.isfinite(grad[0, [0, 2]]).all() and torch.isnan(grad[0, 1]).all()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V,k", [(1, 1), (65, 65), (601, 200), (2047, 100), (4100, 3)])
+def test_many_short_rows(dtype, V, k):
+    """Rows that a wave each reads, some masked, in a slice that starts anywhere."""
+    need("cuda")
+    R = 2049
+    x = make_logits(1, R, V + 3, dtype, "cuda")[..., 1:V + 1]
+    g = torch.Generator().manual_seed(6)
+    mask = (torch.rand(1, R, generator=g) < 0.8).to("cuda")
+    up = torch.randn(1, R, generator=g).to("cuda") * (64.0 if dtype == torch.float16 else 1.0)
+    check_policy(x, *make_rollout(x), mask, reduction="none", up=up)
+    values, indices, lse = make_record(x, k, 1.5)
+    x[0, ~mask[0]] = float("nan")
+    check_distill(x, values, indices, lse, 1.5, mask, "none", up)
+    check_distill(x, values, indices, None, 1.5, mask, "none", up)
+
+
 # ------------------------------------------------------------------ preference
 def preference_oracle(logits, targets, ref, beta, eps, ignore):
     N = logits.shape[0] // 2
