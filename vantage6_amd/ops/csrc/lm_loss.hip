@@ -703,6 +703,12 @@ __global__ void __launch_bounds__(kThreads)
   const int nv = cut.nv;
   char* dxv = dx + cut.head * X::size;
   float a = kp.coef[r];
+  long long at = -1;  // the thread's place of the record
+  float p = 0.f;
+  if (!ONE && tid < pl.K) {
+    at = place(pl, (long long)r * pl.K + tid) - v0;
+    p = kp.p[(long long)r * pl.K + tid];
+  }
   if (a != 0.f) {
     if (up.per == LM_UP_ALL)
       a *= up.g[0] * *kp.inv;
@@ -721,15 +727,13 @@ __global__ void __launch_bounds__(kThreads)
   const LmStat st = kp.stat[r];
   const float c = in.c, mb = st.mb, w = a * st.w;
   const long long target = ONE ? place(pl, r) - v0 : -1;
-  // a place of the record in this segment, and what goes there. The same
-  // index twice adds both probabilities, and both threads write one value.
-  long long at = -1;
+  // what goes to a place in this segment. The same index twice adds both
+  // probabilities, and both threads write one value.
   float there = 0.f;
   if (!ONE) {
     if (tid < pl.K) {
-      at = place(pl, (long long)r * pl.K + tid) - v0;
       s_idx[tid] = at;
-      s_p[tid] = kp.p[(long long)r * pl.K + tid];
+      s_p[tid] = p;
       if (at >= n) at = -1;
     }
     __syncthreads();
@@ -753,8 +757,10 @@ __global__ void __launch_bounds__(kThreads)
     }
     store16<NT>(dxv + (long long)ig * 16, X::close(f));
   };
+  // rounds that a whole wave has, then what is left in one more (vector by
+  // vector 60000 rows of 5001 bf16 take 208 us, so 176)
   int i = tid;
-  for (; i + (Q - 1) * kThreads < nv; i += Q * kThreads) {
+  for (; (i | 63) + (Q - 1) * kThreads < nv; i += Q * kThreads) {
     u32x4 raw[Q];
 #pragma unroll
     for (int g = 0; g < Q; ++g)
@@ -762,7 +768,16 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
     for (int g = 0; g < Q; ++g) put(raw[g], i + g * kThreads);
   }
-  for (; i < nv; i += kThreads) put(load16<true>(xv + (long long)i * 16), i);
+  if (i < nv) {
+    u32x4 raw[Q];
+#pragma unroll
+    for (int g = 0; g < Q; ++g)
+      if (i + g * kThreads < nv)
+        raw[g] = load16<true>(xv + (long long)(i + g * kThreads) * 16);
+#pragma unroll
+    for (int g = 0; g < Q; ++g)
+      if (i + g * kThreads < nv) put(raw[g], i + g * kThreads);
+  }
   if (tid < cut.loose) {
     const int j = loose_at<TY>(cut, tid);
     float f = w * exp2_hw((X::one(x + j * X::size) - mb) * c);
@@ -1094,10 +1109,11 @@ long long bytes_of(const LmRows& in) {
 // 30522: 4.5 us, with 1024 5.8; 200 of 128256 14, with 256 too), of grad 2048
 // (700 rows of 30522 16 us, with 512 18).
 constexpr int kStatBlocks = 512, kGradBlocks = 2048;
-// A segment's most: of stats what its bits in LDS allow; of grad four rounds of
-// loads a thread while the cache holds the logits (4096 rows of 30522 fp16 72
-// us, in one round 75), else one (2048 rows of 128256 151 us, in four 159).
-constexpr int kStatSeg = 131072, kGradSegBytes = 65536, kGradSegFar = 16384;
+// A segment's most: of stats what its bits in LDS allow; of grad two rounds of
+// loads a thread while the cache holds the logits (4096 rows of 30522 fp16 69
+// us, in one round 72, in four 71), else one (2048 rows of 128256 150 us, in two
+// 155, in four 159, half a round 165).
+constexpr int kStatSeg = 131072, kGradSegBytes = 32768, kGradSegFar = 16384;
 // Threads of a block of topk: 512, or 1024 where there are no more rows than
 // CUs and each is long. At 1024 rows of 128256 both take 56 us (256 threads
 // 64), at 4000 rows of 8000 512 take 44 us and 1024 take 72, at 100 rows of
