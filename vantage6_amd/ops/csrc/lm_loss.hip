@@ -758,7 +758,7 @@ __global__ void __launch_bounds__(kThreads)
     store16<NT>(dxv + (long long)ig * 16, X::close(f));
   };
   // rounds that a whole wave has, then what is left in one more (vector by
-  // vector 60000 rows of 5001 bf16 take 208 us, so 176)
+  // vector 60000 rows of 5001 bf16 take 220 us, so 200)
   int i = tid;
   for (; (i | 63) + (Q - 1) * kThreads < nv; i += Q * kThreads) {
     u32x4 raw[Q];
@@ -1088,11 +1088,16 @@ __global__ void __launch_bounds__(THREADS)
 
 int div_up(long long a, long long b) { return (int)((a + b - 1) / b); }
 
+// Blocks that a pass asks for at least, splitting rows: 64 rows of 30522 take
+// 4.5 us in stats, with 1024 5.8, and as fp32 5.1 in grad, with 2048 6.0; 200
+// rows of 128256 14 in stats, with 256 too.
+constexpr int kBlocks = 512;
+
 // Splits of a row over blocks: enough blocks to fill the chip, none with less
 // than one vector per thread.
-int splits_for(const LmRows& in, int blocks, int seg_most, int* seg) {
+int splits_for(const LmRows& in, int seg_most, int* seg) {
   const int per = kThreads * (in.type == LM_FP32 ? 4 : 8);
-  int s = div_up(blocks, in.R);
+  int s = div_up(kBlocks, in.R);
   s = std::min(s, std::max(1, div_up(in.V, per)));
   s = std::max(s, div_up(in.V, seg_most));
   // whole vectors per thread, so that segments start where vectors do
@@ -1105,10 +1110,6 @@ long long bytes_of(const LmRows& in) {
   return (long long)in.R * in.V * (in.type == LM_FP32 ? 4 : 2);
 }
 
-// Blocks that a pass asks for at least, splitting rows: of stats 512 (64 rows of
-// 30522: 4.5 us, with 1024 5.8; 200 of 128256 14, with 256 too), of grad 2048
-// (700 rows of 30522 16 us, with 512 18).
-constexpr int kStatBlocks = 512, kGradBlocks = 2048;
 // A segment's most: of stats what its bits in LDS allow; of grad two rounds of
 // loads a thread while the cache holds the logits (4096 rows of 30522 fp16 69
 // us, in one round 72, in four 71), else one (2048 rows of 128256 150 us, in two
@@ -1122,13 +1123,14 @@ constexpr int kTopkFewRows = 256, kTopkLongRow = 8192;  // vectors
 
 // What the pass over a row leaves in the 256 MB cache behind the L2, the pass
 // of the gradient need not fetch again. At 525 MB of logits a cache that every
-// line goes through keeps little of them: stats + grad take 94 + 178 us, 82 +
-// 196 where all of stats' loads are told not to stay, and 88 + 162 where those
-// of 9 rows of 16 may. At 200 MB all may stay (36 + 60 us, else 37 + 70).
+// line goes through keeps little of them: stats + grad take 97 + 171 us, 83 +
+// 166 where all of stats' loads are told not to stay, and 88 + 150 where those
+// of 9 rows of 16 may. At 203 MB all may stay (32 + 53 us, else 31 + 66).
 constexpr long long kKeepBytes = 300 * kMB;
 // A gradient of this size is gone from the caches before anyone reads it, and
-// written past them it leaves them the logits (81 MB: 28 against 32 us, 203
-// MB: 59 against 68); a smaller one stays for the product that follows.
+// written past them it leaves them the logits: at 244 MB stats + grad take 49 +
+// 58 us, else 78 + 72; at 163 MB 33 + 40, else 40 + 55; at 81 MB grad 22, else
+// 24. A smaller one stays for the product that follows.
 constexpr long long kStreamGrad = 64 * kMB;
 // topk reads a row once and its best lines again: streamed at 263 MB 56 against
 // 60 us, at 78 MB 22 against 20.
@@ -1143,7 +1145,7 @@ template <int TY>
 void grad_of(const LmRows& in, const LmPlaces& pl, const LmKeep& kp,
              const LmUp& up, void* dx, hipStream_t s) {
   int seg;
-  const int splits = splits_for(in, kGradBlocks, grad_seg(in), &seg);
+  const int splits = splits_for(in, grad_seg(in), &seg);
   const dim3 grid((unsigned)in.R * splits);
   const bool nt = bytes_of(in) > kStreamGrad;
   auto kernel = kp.p ? (nt ? lm_grad_kernel<TY, false, true> : lm_grad_kernel<TY, false, false>)
@@ -1177,7 +1179,7 @@ template <int TY>
 void stats_of(const LmRows& in, const LmPlaces& pl, const LmTeacher& te,
               const LmWork& w, const LmKeep& kp, hipStream_t s) {
   int seg;
-  const int splits = splits_for(in, kStatBlocks, kStatSeg, &seg);
+  const int splits = splits_for(in, kStatSeg, &seg);
   if (in.R >= kWaveRows && in.V / Ty<TY>::N <= kWaveVectors)
     stats_with<TY, 64>(in, pl, te, w, kp, splits, seg, s);
   else
@@ -1230,12 +1232,12 @@ void stats(const LmRows& in, const LmPlaces& pl, const LmTeacher& te,
 
 int lm_stats_splits(const LmRows& in) {
   int seg;
-  return splits_for(in, kStatBlocks, kStatSeg, &seg);
+  return splits_for(in, kStatSeg, &seg);
 }
 
 int lm_grad_splits(const LmRows& in) {
   int seg;
-  return splits_for(in, kGradBlocks, grad_seg(in), &seg);
+  return splits_for(in, grad_seg(in), &seg);
 }
 
 int lm_group(int splits) {
