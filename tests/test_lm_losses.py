@@ -816,6 +816,31 @@ def test_rows_of_several_segments(dtype):
 
 
 @pytest.mark.gpu
+def test_most_rows():
+    """2**22 - 1 rows, the most of a call: as its first 6141, which it repeats."""
+    need("cuda")
+    n, times, V = 6141, 683, 3
+    assert n * times == 2 ** 22 - 1
+    base = make_logits(1, n, V, torch.float32, "cuda")
+    x = base.repeat(1, times, 1).requires_grad_(True)
+    top, want = topk_logits(x, 2), topk_logits(base, 2)
+    for got, part in zip(top, want):
+        assert torch.equal(got.unflatten(1, (times, n)), part[:, None].expand(
+            1, times, n, *part.shape[2:]))
+    values, indices, lse = make_record(base, 2, 1.0)
+    small, grad = check_distill(base, values, indices, lse, reduction="none")
+    loss = distill_loss(x, values.repeat(1, times, 1), indices.repeat(1, times, 1),
+                        lse.repeat(1, times), reduction="none")
+    got, = torch.autograd.grad(loss.sum(), x)
+    for big, part in ((loss, small), (got, grad)):
+        # both are within their tolerances of one value
+        torch.testing.assert_close(big.detach().unflatten(1, (times, n)),
+                                   part[:, None].expand(1, times, *part.shape[1:]),
+                                   rtol=2.0 ** -21, atol=4 * LP)
+    check_policy(x.detach(), *make_rollout(x.detach()))
+
+
+@pytest.mark.gpu
 def test_no_grad_and_inference_mode():
     need("cuda")
     x = make_logits(4, 9, 515, torch.bfloat16, "cuda").requires_grad_(True)
