@@ -119,6 +119,26 @@ def test_topk_ties_and_masks(device, dtype):
         check_topk(x[:, V - v:].to(device), 12)
 
 
+@pytest.mark.parametrize("device", CPU_GPU)
+@pytest.mark.parametrize("dtype", TYPES)
+def test_topk_infinite_logits(device, dtype):
+    """A logit of +inf and no NaN beside it: the logsumexp is +inf, at any
+    place of a row, alone, several times, and beside -inf."""
+    need(device)
+    V = 5003
+    x = make_logits(1, 6, V, dtype, "cpu")[0]
+    x[0, 4500] = x[1, V - 1] = x[2, V - 700] = float("inf")
+    x[3] = float("inf")
+    x[4] = float("-inf")
+    x[4, V - 300] = float("inf")
+    x[5, V - 200] = float("inf")
+    x[5, V - 100] = float("nan")  # with a NaN: a NaN
+    for v in (V, 700, 1):  # a row in lines or in vectors, one kept whole, one logit
+        for k, t in ((1, 1.0), (12, 2.0), (40, 0.5)):
+            if k <= v:
+                check_topk(x[:, V - v:].to(device), k, t)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("V,k", [(600, 256), (2100, 200), (4096, 256), (4097, 256), (8200, 256),

@@ -973,7 +973,9 @@ __global__ void __launch_bounds__(THREADS)
     a = wave_join(a, in);
     if (tid == 64) {
       s_run = a;
-      odd = a.s != a.s;  // a NaN hides from fmaxf, but not from the sum
+      // a NaN hides from fmaxf, but not from the sum, nor does a +inf, whose
+      // difference from itself is one
+      odd = a.s != a.s;
     }
   }
   __syncthreads();
@@ -1066,7 +1068,7 @@ __global__ void __launch_bounds__(THREADS)
     nc = n_cand;
   }
   // the last wave has the fewest candidates; a row of -inf: log 0
-  if (tid == THREADS - 1)
+  if (!odd && tid == THREADS - 1)
     lse[r] = (float)((double)s_run.m / temperature + log((double)s_run.s));
   // rank by counting, 8 lanes to a candidate
   for (int i0 = 0; i0 < nc; i0 += THREADS / 8) {
@@ -1082,6 +1084,8 @@ __global__ void __launch_bounds__(THREADS)
       const long long at = (long long)r * k + rank;
       indices[at] = place_of(mine);
       X::put(values + at * X::size, logit_of(mine));
+      // a NaN ranks first, and without one the row's +inf is its logsumexp
+      if (odd && rank == 0) lse[r] = logit_of(mine);
     }
   }
 }
