@@ -634,6 +634,28 @@ def test_policy_masks(device):
 
 
 @pytest.mark.parametrize("device", CPU_GPU)
+def test_policy_kl_without_weight(device):
+    """With a coefficient of 0 the KL is reported only, and one that passes the
+    largest number changes neither loss nor gradient."""
+    need(device)
+    x = make_logits(1, 4, 64, torch.float32, device)
+    actions = torch.tensor([[3, 9, 20, 63]], device=device)
+    x[0, 1, 9] = -1000.0  # exp(999) is none in 64 bits either
+    x[0, 2, 20] = torch.finfo(torch.float32).min
+    old = softmax64(x).gather(-1, actions.cpu()[..., None])[..., 0].float().to(device)
+    adv = torch.tensor([[1.0, -0.5, 2.0, -1.0]], device=device)
+    ref = torch.full((1, 4), -1.0, device=device)
+    x.requires_grad_(True)
+    for reduction in ("none", "mean"):
+        got = policy_loss(x, actions, old, adv, ref, kl_coef=0.0, reduction=reduction)
+        want = policy_loss(x, actions, old, adv, reduction=reduction)
+        assert torch.isfinite(want.loss).all() and torch.equal(got.loss, want.loss)
+        a, b = (torch.autograd.grad(o.loss.sum(), x)[0] for o in (got, want))
+        assert torch.isfinite(b).all() and torch.equal(a, b)
+        assert torch.isinf(got.kl[0, 1:3]).all() and torch.isfinite(got.kl[0, [0, 3]]).all()
+
+
+@pytest.mark.parametrize("device", CPU_GPU)
 @pytest.mark.parametrize("dtype", TYPES)
 def test_masked_logits(device, dtype):
     """-inf (a padded head) and the type's lowest value in a row: no gradient

@@ -607,8 +607,11 @@ __global__ void __launch_bounds__(kThreads)
     if (po.ref_lp) {
       const double d = (double)po.ref_lp[r] - lp, e = expm1(d);
       kl = e - d;
-      loss += po.kl_coef * kl;
-      by_lp -= po.kl_coef * e;
+      // without weight it is reported only: it may be +inf, and 0 * inf a NaN
+      if (po.kl_coef != 0.0) {
+        loss += po.kl_coef * kl;
+        by_lp -= po.kl_coef * e;
+      }
     }
   }
   if (lead) {

@@ -105,7 +105,8 @@ def policy_loss(logits: torch.Tensor, actions: torch.Tensor,
 
     ``logits`` is ``[..., V]``; ``actions`` the sampled tokens, ``old_logps``
     their log-probabilities when they were sampled, ``advantages``, and
-    ``ref_logps`` the frozen model's (None: no KL term), all ``[...]``.
+    ``ref_logps`` the frozen model's (None: no KL term; with ``kl_coef`` 0 the
+    KL is reported only), all ``[...]``.
     Tokens where ``mask`` is False do not count: their logits are not read,
     loss, ``logps``, ``kl`` and gradient are exactly 0. The gradient passes
     where the ratio sits on a border of the clip. An action outside [0, V)
@@ -149,7 +150,8 @@ def policy_loss(logits: torch.Tensor, actions: torch.Tensor,
     if ref_logps is not None:
         d = torch.where(live, ref_logps, 0).double() - lp
         kl = torch.expm1(d) - d
-        rows = rows + kl_coef * kl
+        if kl_coef:  # else it is reported only: it may be +inf
+            rows = rows + kl_coef * kl
     rows = torch.where(live, rows, 0.0)
     loss = reduce_rows(rows, live, reduction)
     if logits.dtype != torch.float64:
