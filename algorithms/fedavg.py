@@ -28,8 +28,8 @@ from vantage6_amd.parallel.fedavg import FedAvgConfig, FedAvgTrainer
 # shared helpers
 # --------------------------------------------------------------------------
 # what another model or a rollout measured: compared with, not computed in
-_EXACT_KEYS = frozenset(("teacher_values", "teacher_lse", "ref_logps",
-                         "old_logps", "advantages"))
+_EXACT_KEYS = frozenset(("teacher_values", "teacher_lse", "teacher_temperature",
+                         "ref_logps", "old_logps", "advantages"))
 
 
 def make_batches(dataset: dict, batch_size: int, device, dtype=torch.bfloat16,
@@ -97,6 +97,11 @@ def fit_rounds(
     if dp and objective is not None:
         raise ValueError("DP-SGD clips per-sample next-token losses only: no "
                          f"objective {objective!r}")
+    if objective == "distill" and {"teacher_lse", "teacher_temperature"} <= set(dataset):
+        t = (objective_options or {}).get("temperature", 1.0)
+        if (dataset["teacher_temperature"] != t).any():
+            raise ValueError("the dataset's teacher_lse is not of the "
+                             f"objective's temperature {t}")
     net, loss_fn = _build(model, model_kwargs, device, objective=objective,
                           objective_options=objective_options)
     batches = make_batches(dataset, batch_size, device, seed=17 + comm.rank)

@@ -1176,6 +1176,43 @@ def test_fit_rounds_with_an_objective(device, objective):
     assert all(batch[k].dtype == data[k].dtype for k in data)  # measured values stay exact
 
 
+@pytest.mark.parametrize("device", CPU_GPU)
+def test_record_of_another_temperature(device):
+    """A record's logsumexp holds at its temperature alone: the trainer refuses
+    another, and a batch of it has a NaN for a loss. Without the logsumexp the
+    record serves any."""
+    need(device)
+    from algorithms.fedavg import fit_rounds, make_batches
+    from vantage6_amd.models import build_model, model_loss, teacher_record
+
+    torch.manual_seed(1)
+    kw = dict(TINY["llama_1b"])
+    model = build_model("llama_1b", device=device, **kw)
+    ids = torch.randint(0, kw["vocab"], (6, 8), generator=torch.Generator().manual_seed(2))
+    for made in (1.0, 0.7):
+        record = teacher_record(model, ids.to(device), 5, temperature=made)
+        assert record["teacher_temperature"].shape == (6,)
+        data = {"input_ids": ids, **{k: v.cpu() for k, v in record.items()}}
+        batch = next(make_batches(data, 4, device))
+        lse = batch.pop("teacher_lse")
+        for used in (1.0, 0.7):
+            loss = model_loss("llama_1b", "distill", temperature=used)
+            assert torch.isfinite(loss(model, batch))
+            got = loss(model, {**batch, "teacher_lse": lse})
+            assert torch.isfinite(got) if used == made else torch.isnan(got)
+            options = dict(model="llama_1b", model_kwargs=kw, rounds=1, local_steps=1, batch_size=4,
+                           device=torch.device(device), objective="distill")
+            if used == 1.0:  # the default
+                run = lambda: fit_rounds(data, **options)
+            else:
+                run = lambda: fit_rounds(data, objective_options={"temperature": used}, **options)
+            if used == made:
+                assert math.isfinite(run()["final_loss"])
+            else:
+                with pytest.raises(ValueError, match="temperature"):
+                    run()
+
+
 def test_objective_refusals():
     from algorithms.fedavg import fit_rounds
     from vantage6_amd.models import model_loss

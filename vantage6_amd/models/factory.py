@@ -51,14 +51,19 @@ def _lm_logits(model, ids):
 def _distill_objective(options) -> Callable:
     """Batch: ``input_ids`` [N, S] and the teacher's record of every position,
     ``teacher_values`` and ``teacher_indices`` [N, S, k], optionally
-    ``teacher_lse`` and ``mask`` [N, S]."""
+    ``teacher_lse`` and ``mask`` [N, S]. With ``teacher_temperature`` [N] a
+    ``teacher_lse`` of another temperature than the loss's makes the loss NaN,
+    as a device cannot raise."""
     def loss(model, batch):
         from ..ops.distill import distill_loss
 
+        lse = batch.get("teacher_lse")
+        if lse is not None and "teacher_temperature" in batch:
+            same = batch["teacher_temperature"] == options.get("temperature", 1.0)
+            lse = torch.where(same[:, None], lse, float("nan"))
         return distill_loss(
             _lm_logits(model, batch["input_ids"]), batch["teacher_values"],
-            batch["teacher_indices"], batch.get("teacher_lse"),
-            mask=batch.get("mask"), **options)
+            batch["teacher_indices"], lse, mask=batch.get("mask"), **options)
 
     return loss
 
@@ -106,12 +111,16 @@ _OBJECTIVES = {"distill": _distill_objective, "preference": _preference_objectiv
 @torch.no_grad()
 def teacher_record(model, input_ids, k: int = 64, temperature: float = 1.0) -> dict:
     """What a station publishes of its model's answers to ``input_ids``: the
-    entries that the "distill" objective's batches hold."""
+    entries that the "distill" objective's batches hold. ``teacher_lse`` is of
+    ``temperature``, the objective's own; ``teacher_temperature`` [N] says so."""
     from ..ops.distill import topk_logits
 
     top = topk_logits(_lm_logits(model, input_ids), k, temperature)
     return {"teacher_values": top.values, "teacher_indices": top.indices,
-            "teacher_lse": top.logsumexp}
+            "teacher_lse": top.logsumexp,
+            "teacher_temperature": torch.full(
+                input_ids.shape[:1], float(temperature), dtype=torch.float64,
+                device=top.values.device)}
 
 
 def model_loss(name: str, objective: str | None = None, **options) -> Callable:
