@@ -316,6 +316,27 @@ def test_distill_odd_records(device, tail):
 
 
 @pytest.mark.parametrize("device", CPU_GPU)
+@pytest.mark.parametrize("tail", [False, True])
+def test_distill_layouts(device, tail):
+    """Slices, one row, more dimensions, rows that are one; records of another
+    type, not contiguous, in another order; masks that are broadcast."""
+    need(device)
+    x = make_logits(3, 7, 515, torch.float32, device)
+    for view in (x[:, :-1], x[:, 1:, :512], x[:, :6, 3:], x[0, 1:], x[1, 2],
+                 x.transpose(0, 1)[1:], x[:, :6].reshape(3, 2, 3, 515),
+                 x[:1].expand(3, 7, 515), x[..., ::2]):
+        values, indices, lse = make_record(view, 9, 1.0, tail=tail)
+        values, indices = values.flip(-1)[..., ::2], indices.flip(-1)[..., ::2]
+        assert not values.is_contiguous() or values.dim() == 1
+        for v, L in ((values, lse), (values.bfloat16(), lse), (values.half(), lse),
+                     (values.double(), None if lse is None else lse.double())):
+            mask = None
+            if view.dim() > 1:
+                mask = (torch.arange(view.shape[-2]) != 1).to(device).expand(view.shape[:-1])
+            check_distill(view, v, indices, L, 1.0, mask)
+
+
+@pytest.mark.parametrize("device", CPU_GPU)
 def test_distill_whole_row_in_the_record(device):
     need(device)
     x = make_logits(1, 3, 200, torch.float32, device)
