@@ -619,6 +619,52 @@ def test_policy(device, dtype, shape):
                  up=torch.tensor(scale, device=device))
 
 
+def check_policy_grad(got, grad, by_lp, big, q, actions):
+    """got against ``grad`` = by_lp (onehot - q). An error of by_lp, at most
+    GRAD of ``big``, moves a place by |onehot - q| of it, one of q by q of it:
+    1 - q is allowed at the action alone."""
+    one = torch.zeros_like(q).scatter_(-1, actions.cpu().long()[..., None], 1.0)
+    check_grad(got, grad, big, (one - q).abs() + q)
+    assert (got.cpu()[by_lp == 0] == 0).all()
+
+
+@pytest.mark.parametrize("device", CPU_GPU)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", SHAPES)
+def test_policy_gradient_of_every_logit(device, dtype, shape):
+    """The gradient of the sum, so that the small ones are no denormals."""
+    need(device)
+    B, T, V = shape
+    base = make_logits(B, T, V + 2, dtype, device)
+    up = 512.0 if dtype == torch.float16 else 1.0
+    for view in (base[..., :V].contiguous(), base[..., 1:V + 1]):
+        actions, old, adv, ref = make_rollout(view)
+        x = view.detach().requires_grad_(True)
+        out = policy_loss(x, actions, old, adv, ref, kl_coef=0.05, reduction="sum")
+        got, = torch.autograd.grad(out.loss, x, torch.tensor(up, device=device))
+        _, _, _, grad, by_lp, q, _ = policy_oracle(view, actions, old, adv, ref, None, 0.2, 0.2, 0.05)
+        big = by_lp.abs() + adv.cpu().double().abs() * 2 + 0.05 * 3
+        check_policy_grad(got, grad * up, by_lp, big * up, q, actions)
+
+
+@pytest.mark.parametrize("V", [613, 4099, 30522, 128256])
+def test_policy_gradient_check_sees_small_probabilities(V):
+    """The check itself: a gradient that lacks what is below q = 1e-4, or one
+    place of it, is not accepted."""
+    x = make_logits(1, 3, V, torch.float32, "cpu")
+    actions, old, adv, ref = make_rollout(x)
+    _, _, _, grad, by_lp, q, _ = policy_oracle(x, actions, old, adv, ref, None, 0.2, 0.2, 0.05)
+    assert (by_lp != 0).all()  # no row is clipped
+    big = by_lp.abs() + adv.double().abs() * 2 + 0.05 * 3
+    right = (grad, by_lp, big, q, actions)
+    check_policy_grad(grad.float(), *right)
+    away = torch.ones_like(q, dtype=torch.bool).scatter_(-1, actions[..., None], False)
+    for lost in (away & (q < 1e-4), away & (torch.arange(V) == V - 1)):
+        assert lost.any()
+        with pytest.raises(AssertionError):
+            check_policy_grad(grad.masked_fill(lost, 0.0).float(), *right)
+
+
 @pytest.mark.parametrize("device", CPU_GPU)
 @pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
 def test_policy_reductions_and_layouts(device, reduction):
