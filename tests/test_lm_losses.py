@@ -317,6 +317,22 @@ def test_distill_odd_records(device, tail):
 
 @pytest.mark.parametrize("device", CPU_GPU)
 @pytest.mark.parametrize("tail", [False, True])
+def test_distill_empty_records_hold_anything(device, tail):
+    """Rows whose record holds nothing, whatever their logits are."""
+    need(device)
+    x = make_logits(1, 5, 700, torch.float32, device)
+    values, indices, lse = make_record(x, 6, 1.0, tail=tail)
+    indices[0, 1], values[0, 3] = -1, float("-inf")
+    want, grad = check_distill(x, values, indices, lse)
+    x[0, 1], x[0, 3, ::2], x[0, 3, 1::2] = float("nan"), float("inf"), float("-inf")
+    x.requires_grad_(True)
+    loss = distill_loss(x, values, indices, lse)
+    got, = torch.autograd.grad(loss, x)
+    assert torch.equal(loss.detach(), want) and torch.equal(got, grad)
+
+
+@pytest.mark.parametrize("device", CPU_GPU)
+@pytest.mark.parametrize("tail", [False, True])
 def test_distill_layouts(device, tail):
     """Slices, one row, more dimensions, rows that are one; records of another
     type, not contiguous, in another order; masks that are broadcast."""
