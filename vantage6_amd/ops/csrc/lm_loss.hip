@@ -760,8 +760,8 @@ __global__ void __launch_bounds__(kThreads)
     }
     store16<NT>(dxv + (long long)ig * 16, X::close(f));
   };
-  // rounds that a whole wave has, then what is left in one more (vector by
-  // vector 60000 rows of 5001 bf16 take 220 us, so 200)
+  // rounds that a whole wave has, then what is left in one more (60000 rows of
+  // 5001 bf16: vector by vector 208 us, so 176; with a record 220 and 200)
   int i = tid;
   for (; (i | 63) + (Q - 1) * kThreads < nv; i += Q * kThreads) {
     u32x4 raw[Q];
@@ -1161,8 +1161,9 @@ void grad_of(const LmRows& in, const LmPlaces& pl, const LmKeep& kp,
 }
 
 // Many short rows take a wave each: a block's start, its joins through LDS and
-// its end outweigh such a row. 8192 rows of 600 bf16 8 us, in blocks of 256
-// threads 23; 60000 of 5001 112 and 157; 4096 of 16000 24 and 25. A wave alone is
+// its end outweigh such a row. This pass alone, again and again: 8192 rows of 600
+// bf16 8 us, in blocks of 256 threads 23; 60000 of 5001 112 and 157 (131 behind a
+// gradient's pass); 4096 of 16000 24 and 25. A wave alone is
 // behind with few rows (512 of 5001 fp32 5.2 and 4.4 us, 1024 of 8200 8.8 and
 // 6.8) and with longer ones (8192 of 30522 bf16 with a record 86 and 82).
 constexpr int kWaveRows = 2048, kWaveVectors = 2048;

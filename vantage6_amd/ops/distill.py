@@ -77,9 +77,10 @@ def distill_loss(logits: torch.Tensor, teacher_values: torch.Tensor,
     in any order, ``teacher_lse`` ``[...]`` or None (see above); ``logits /
     temperature`` is what both sides are compared at. An entry with a negative
     index is absent, one with a value of -inf has no probability; the same
-    index twice adds up. A row is ignored (loss 0, gradient exactly 0, its
-    logits not read) where ``mask`` is False or its record holds nothing.
-    An index of V or more makes the row's loss and gradient NaN.
+    index twice adds up. A row is ignored (loss 0, gradient exactly 0, whatever
+    its logits hold) where ``mask`` is False, and then its logits are not read,
+    or where its record holds nothing. An index of V or more makes the row's
+    loss and gradient NaN.
 
     ``reduction``: "mean" over the rows that count, "sum", or "none" (a loss
     per row). The record is a constant of the loss."""

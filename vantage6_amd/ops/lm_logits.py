@@ -1,7 +1,7 @@
 """What the losses over language-model logits share (csrc/lm_loss.hip).
 
-Argument checks, the layout that the kernels read, and the row softmax of
-the CPU path. The kernels take ``[V]``, ``[T, V]`` or ``[B, T, V]`` logits
+Argument checks, the layout that the kernels read, and the CPU path's types
+and reductions. The kernels take ``[V]``, ``[T, V]`` or ``[B, T, V]`` logits
 whose rows may lie anywhere (a slice ``logits[:, :-1]`` is read in place);
 more dimensions are folded into ``B``, and logits whose last dimension is
 not contiguous are copied once. A call takes up to 2**22 - 1 rows.
