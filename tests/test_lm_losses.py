@@ -980,6 +980,28 @@ def test_no_grad_and_inference_mode():
             assert topk_logits(x.clone(), 3).values.shape == (4, 9, 3)
 
 
+@pytest.mark.parametrize("device", CPU_GPU)
+def test_records_and_rollouts_of_inference_mode(device):
+    """A teacher answers and a rollout is sampled in inference mode; what they
+    give trains a model outside of it."""
+    need(device)
+    x = make_logits(4, 9, 515, torch.float32, device).requires_grad_(True)
+
+    def made():
+        record = topk_logits(x.detach() * 1.5, 7, 2.0)
+        return make_pairs(2, 9, 515, device), make_rollout(x), record[:2], record[2]
+
+    def step(pairs, rollout, record, lse):
+        losses = all_losses(x, pairs, rollout, record, lse)
+        return [l.detach() for l in losses] + [torch.autograd.grad(l, x)[0] for l in losses]
+
+    want = step(*made())
+    with torch.inference_mode():
+        args = made()
+    assert args[2][1].is_inference() and args[1][0].is_inference()
+    assert all(torch.equal(a, b) for a, b in zip(want, step(*args)))
+
+
 @pytest.mark.gpu
 def test_changed_logits_are_noticed():
     """The gradient is made from the logits that the loss saw, or not at all."""

@@ -653,6 +653,12 @@ static torch::Tensor lm_loss_out(const torch::Tensor& x, at::IntArrayRef each,
   return loss;
 }
 
+// Places that the backward pass reads again. Those of a record or a rollout made
+// in inference mode cannot be saved as they are.
+static torch::Tensor lm_savable(const torch::Tensor& idx) {
+  return idx.is_inference() && !c10::InferenceMode::is_enabled() ? idx.clone() : idx;
+}
+
 static void lm_set_idx(LmPlaces* pl, const torch::Tensor& idx) {
   TORCH_CHECK(idx.scalar_type() == torch::kLong || idx.scalar_type() == torch::kInt,
               "indices must be int64 or int32");
@@ -723,7 +729,7 @@ struct LmDistillFn : public torch::autograd::Function<LmDistillFn> {
     TORCH_CHECK(idx.device() == x.device() && values.device() == x.device(),
                 "distill: the record must be on the logits' device");
     c10::DeviceGuard guard(x.device());
-    if (!idx.is_contiguous()) idx = idx.contiguous();
+    idx = lm_savable(idx.is_contiguous() ? idx : idx.contiguous());
     if (!values.is_contiguous()) values = values.contiguous();
     if (lse) lse = lm_per_row(*lse, x, torch::kFloat32, "teacher_lse");
     if (mask) mask = lm_per_row(*mask, x, torch::kBool, "mask");
@@ -764,7 +770,7 @@ struct LmPolicyFn : public torch::autograd::Function<LmPolicyFn> {
                                double kl_coef, int64_t reduction) {
     LmRows in = lm_rows(x, 1.0);
     c10::DeviceGuard guard(x.device());
-    actions = lm_per_row(actions, x, torch::kLong, "actions");
+    actions = lm_savable(lm_per_row(actions, x, torch::kLong, "actions"));
     old_lp = lm_per_row(old_lp, x, torch::kFloat32, "old_logps");
     adv = lm_per_row(adv, x, torch::kFloat32, "advantages");
     if (ref_lp) ref_lp = lm_per_row(*ref_lp, x, torch::kFloat32, "ref_logps");
@@ -811,7 +817,7 @@ struct LmPreferenceFn : public torch::autograd::Function<LmPreferenceFn> {
     TORCH_CHECK(ref.device() == x.device() && ref.dim() == 1 &&
                 ref.size(0) == x.size(0), "preference: ref_logps must be [2N]");
     c10::DeviceGuard guard(x.device());
-    targets = lm_per_row(targets, x, torch::kLong, "targets");
+    targets = lm_savable(lm_per_row(targets, x, torch::kLong, "targets"));
     if (ref.scalar_type() != torch::kDouble && ref.scalar_type() != torch::kFloat32)
       ref = ref.to(torch::kFloat32);
     if (!ref.is_contiguous()) ref = ref.contiguous();
