@@ -388,6 +388,25 @@ def test_distill_index_outside_is_nan(device):
     assert torch.isfinite(grad[0, [0, 2]]).all() and torch.isnan(grad[0, 1]).all()
 
 
+@pytest.mark.parametrize("device", CPU_GPU)
+@pytest.mark.parametrize("tail", [False, True])
+def test_distill_unlikely_index_outside_is_nan(device, tail):
+    """An index outside the row is one however small its probability; a value
+    of -inf there has none."""
+    need(device)
+    x = make_logits(1, 4, 64, torch.float32, device)
+    values, indices, lse = make_record(x, 4, 1.0, tail=tail)
+    indices[0, 1:, 2] = 64
+    values[0, 1, 2] = -1e4  # exp of it is 0 in 64 bits too
+    values[0, 2, 2] = float("-inf")
+    values[0, 3] = torch.tensor([3.0, 2.0, -1e30, 1.0], device=device)
+    x.requires_grad_(True)
+    loss = distill_loss(x, values, indices, lse, reduction="none")
+    grad, = torch.autograd.grad(loss.sum(), x)
+    assert torch.isfinite(loss[0, [0, 2]]).all() and torch.isfinite(grad[0, [0, 2]]).all()
+    assert torch.isnan(loss[0, [1, 3]]).all() and torch.isnan(grad[0, [1, 3]]).any(-1).all()
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("V,k", [(1, 1), (65, 65), (601, 200), (2047, 100), (4100, 3)])

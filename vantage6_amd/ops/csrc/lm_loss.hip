@@ -280,9 +280,9 @@ DEVINL void record_of(const LmRows& in, const LmPlaces& pl, const LmTeacher& te,
     if (64 * e >= pl.K) break;
     if (!te.lse) lp[e] -= z;
     double p = v[e] == -INFINITY ? 0.0 : exp(lp[e]);
+    // a place outside the row makes it a NaN, though its p may be 0
+    if (j[e] >= in.V && v[e] != -INFINITY) p = NAN;
     if (p != 0.0) {
-      // a place outside the row makes it a NaN
-      if (j[e] >= in.V) p = NAN;
       const double x = j[e] < in.V
           ? (double)one_of(in.type, (const char*)in.x, x_at + j[e]) : NAN;
       a += p * lp[e];
