@@ -389,6 +389,34 @@ def test_distill_index_outside_is_nan(device):
 
 
 @pytest.mark.parametrize("device", CPU_GPU)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("t", [1.0, 2.0])
+def test_distill_rows_of_extreme_logits(device, dtype, t):
+    """Rows of the type's lowest or largest value: uniform ones, and not sums of
+    1e38 that cancel to 1e22. A place far below the others counts by its own
+    probability, however small beside the sum of them."""
+    need(device)
+    V = 300
+    fi = torch.finfo(dtype)
+    x = make_logits(1, 4, V, dtype, "cpu")
+    x[0, 0], x[0, 1] = fi.min, fi.max
+    x[0, 2, 100:] = fi.max
+    x[0, 3] = 0.0
+    x[0, 3, 7] = fi.max
+    g = torch.Generator().manual_seed(6)
+    values = torch.randn(1, 4, 9, generator=g).to(dtype)
+    indices = torch.stack([torch.randperm(180, generator=g)[:9] + 110 for _ in range(4)])[None]
+    values[0, 3, 0], indices[0, 3, 0] = 55.0, 7
+    lse = torch.logsumexp(values.double() / t, -1).float() + 0.4
+    x, values, indices, lse = (a.to(device) for a in (x, values, indices, lse))
+    for r in range(4):
+        each = x[:, r:r + 1], values[:, r:r + 1], indices[:, r:r + 1]
+        check_distill(*each, None, t)
+        if r < 3:  # the last row's rest is as impossible as its places
+            check_distill(*each, lse[:, r:r + 1], t)
+
+
+@pytest.mark.parametrize("device", CPU_GPU)
 @pytest.mark.parametrize("tail", [False, True])
 def test_distill_unlikely_index_outside_is_nan(device, tail):
     """An index outside the row is one however small its probability; a value

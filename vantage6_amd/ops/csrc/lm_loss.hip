@@ -236,8 +236,10 @@ DEVINL void block_sum2(double& a, double& b, double2* red) {
 }
 
 // A record's probabilities by one wave, up to 4 of its 256 entries a lane, in
-// 64 bits as 1 - sum p follows. rec = {sum p log p, sum p x, sum p, rest},
-// rest < 0 marks a row without a record.
+// 64 bits as 1 - sum p follows. rec = {sum p log p, sum p (x - x_ref), sum p,
+// x_ref}, sum p < 0 marks a row without a record. x_ref is the largest of the
+// record's logits: sums of p x and of p M would cancel where all of them are the
+// type's lowest value, and leave 1e22 of 1e38.
 DEVINL void record_of(const LmRows& in, const LmPlaces& pl, const LmTeacher& te,
                       int r, float* p_out, double4* rec) {
   constexpr int E = kLmMostK / 64;
@@ -256,7 +258,7 @@ DEVINL void record_of(const LmRows& in, const LmPlaces& pl, const LmTeacher& te,
     m = fmaxf(m, v[e]);
   }
   if (!__any(any)) {
-    if (lane == 0) rec[r] = make_double4(0, 0, 0, -1);
+    if (lane == 0) rec[r] = make_double4(0, 0, -1, 0);
     return;
   }
   double lp[E], z = 0.0;
@@ -274,7 +276,7 @@ DEVINL void record_of(const LmRows& in, const LmPlaces& pl, const LmTeacher& te,
     }
     z = log(wave_sum(z));
   }
-  double a = 0.0, b = 0.0, sum = 0.0;
+  double a = 0.0, b = 0.0, sum = 0.0, x_ref = -FLT_MAX;  // the lane's, so far
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     if (64 * e >= pl.K) break;
@@ -286,16 +288,21 @@ DEVINL void record_of(const LmRows& in, const LmPlaces& pl, const LmTeacher& te,
       const double x = j[e] < in.V
           ? (double)one_of(in.type, (const char*)in.x, x_at + j[e]) : NAN;
       a += p * lp[e];
-      b += p * x;
+      if (x > x_ref) {
+        b += sum * (x_ref - x);
+        x_ref = x;
+      }
+      b += p * (x - x_ref);
       sum += p;
     }
     if (lane + 64 * e < pl.K) p_out[at + lane + 64 * e] = (float)p;
   }
+  const double x_all = wave_max((float)x_ref);
+  b += sum * (x_ref - x_all);
   a = wave_sum(a);
   b = wave_sum(b);
   sum = wave_sum(sum);
-  if (lane == 0)
-    rec[r] = make_double4(a, b, sum, te.lse ? fmax(1.0 - sum, 0.0) : 0.0);
+  if (lane == 0) rec[r] = make_double4(a, b, sum, x_all);
 }
 
 // ------------------------------------------------------------------- stats
@@ -532,8 +539,8 @@ __global__ void __launch_bounds__(kThreads)
   const int at = blockIdx.x * blockDim.x + threadIdx.x, r = at / w.group;
   const bool lead = (at & (w.group - 1)) == 0 && r < in.R;
   const bool on = r < in.R && !ignored(pl, r);
-  const double4 k = on ? w.rec[r] : make_double4(0, 0, 0, -1);
-  const bool live = !(k.w < 0.0);
+  const double4 k = on ? w.rec[r] : make_double4(0, 0, -1, 0);
+  const bool live = !(k.z < 0.0);
   const double t = te.temperature, c = kLog2e / t;
   const Row rest = join_splits(w.part, w.splits, w.group, r, live, c);
   Row top = {0, 0};
@@ -547,14 +554,15 @@ __global__ void __launch_bounds__(kThreads)
     // values and its logsumexp are of the same row
     double tail = 0.0, mass = k.z;
     if (te.lse) {
+      const double p_rest = fmax(1.0 - k.z, 0.0);
       all.m = fmax(rest.m, top.m);
       all.s = rest.s * exp((rest.m - all.m) / t) + top.s * exp((top.m - all.m) / t);
       // no logit outside the record is above -inf: it has no rest
       if (rest.s != 0.0) {
         const double log_rest = (rest.m - all.m) / t + log(rest.s / all.s);
-        if (k.w > 0.0) tail = k.w * (log(k.w) - log_rest);
-        mass += k.w;
-        st.w = (float)((mass * exp(log_rest) - k.w) / rest.s);
+        if (p_rest > 0.0) tail = p_rest * (log(p_rest) - log_rest);
+        mass += p_rest;
+        st.w = (float)((mass * exp(log_rest) - p_rest) / rest.s);
       }
     } else {
       st.w = (float)(mass / all.s);
@@ -562,7 +570,8 @@ __global__ void __launch_bounds__(kThreads)
     st.mb = (float)rest.m;
     st.M = (float)all.m;
     st.mass_S = (float)(mass / all.s);
-    loss = t * t * (k.x - (k.y - k.z * all.m) / t + k.z * log(all.s) + tail);
+    // sum p (log p - log q)
+    loss = t * t * (k.x - (k.y + k.z * (k.w - all.m)) / t + k.z * log(all.s) + tail);
     // d/dx of t^2 KL(x/t); a NaN, of a place outside the row too, is the
     // whole row's
     a = loss == loss ? (float)t : NAN;
