@@ -417,6 +417,28 @@ def test_distill_rows_of_extreme_logits(device, dtype, t):
 
 
 @pytest.mark.parametrize("device", CPU_GPU)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("t", [0.3, 0.05])
+def test_distill_extreme_logits_at_low_temperatures(device, dtype, t):
+    """The type's lowest and largest values, which a division by a temperature
+    below 1 takes past the largest number."""
+    need(device)
+    V = 300
+    fi = torch.finfo(dtype)
+    x = make_logits(1, 4, V, dtype, "cpu", scale=0.3)
+    x[0, 0], x[0, 1] = fi.min, fi.max
+    x[0, 2, 100:] = fi.max
+    x[0, 3, :100] = fi.min
+    g = torch.Generator().manual_seed(6)
+    values = (torch.randn(1, 4, 9, generator=g) * t).to(dtype)
+    indices = torch.stack([torch.randperm(180, generator=g)[:9] + 110 for _ in range(4)])[None]
+    lse = torch.logsumexp(values.double() / t, -1).float() + 0.4
+    args = [a.to(device) for a in (x, values, indices)]
+    check_distill(*args, None, t)
+    check_distill(*args, lse.to(device), t)
+
+
+@pytest.mark.parametrize("device", CPU_GPU)
 @pytest.mark.parametrize("tail", [False, True])
 def test_distill_unlikely_index_outside_is_nan(device, tail):
     """An index outside the row is one however small its probability; a value

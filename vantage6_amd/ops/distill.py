@@ -121,8 +121,9 @@ def _distill_reference(logits, values, indices, lse, t, mask, reduction):
     # rows that do not count are computed on zeros, so that nothing of theirs
     # comes back through a gradient
     on = live[..., None]
-    x = torch.where(on, logits, 0).to(reference_dtype(logits)) / t
-    x = x - x.detach().amax(-1, keepdim=True).clamp_min(torch.finfo(x.dtype).min)
+    x = torch.where(on, logits, 0).to(reference_dtype(logits))
+    top = x.detach().amax(-1, keepdim=True).clamp_min(torch.finfo(x.dtype).min)
+    x = (x - top) / t  # in this order: the type's lowest value stays a number
     at = indices.clamp(0, V - 1)
     inside = torch.zeros(logits.shape, dtype=torch.int32, device=logits.device)
     inside = inside.scatter_add(-1, at, (present & (indices < V)).int()) > 0
