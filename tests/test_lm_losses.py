@@ -786,6 +786,26 @@ def test_policy_masks(device):
 
 
 @pytest.mark.parametrize("device", CPU_GPU)
+def test_policy_impossible_old_tokens(device):
+    """An old log-probability of -inf, or one far below: the ratio passes the
+    largest number, the clip holds the loss and the gradient is 0. Where the
+    advantage is negative nothing holds it."""
+    need(device)
+    x = make_logits(1, 6, 33, torch.float32, device)
+    actions, old, adv, ref = make_rollout(x)
+    old[0, 1], old[0, 2], old[0, 4] = float("-inf"), -1e30, -900.0
+    adv[0] = torch.tensor([1.0, 0.5, 2.0, -1.0, 1.5, 1.0])
+    check_policy(x, actions, old, adv, None, coef=0.0)
+    check_policy(x, actions, old, adv, ref, coef=0.05, reduction="sum")
+    adv[0, 1] = -0.5
+    x.requires_grad_(True)
+    out = policy_loss(x, actions, old, adv, reduction="none")
+    assert out.loss[0, 1].item() == float("inf") and torch.isfinite(out.loss[0, 2:]).all()
+    g, = torch.autograd.grad(out.loss.sum(), x)
+    assert not torch.isfinite(g[0, 1]).any() and torch.isfinite(g[0, 2:]).all()
+
+
+@pytest.mark.parametrize("device", CPU_GPU)
 def test_policy_kl_without_weight(device):
     """With a coefficient of 0 the KL is reported only, and one that passes the
     largest number changes neither loss nor gradient."""

@@ -142,9 +142,12 @@ def policy_loss(logits: torch.Tensor, actions: torch.Tensor,
     live = torch.ones_like(actions, dtype=torch.bool) if mask is None else mask
     lp = _token_logps(logits, actions.long(), live)
     A = torch.where(live, advantages, 0).double()
-    ratio = (lp - torch.where(live, old_logps, 0).double()).exp()
-    held = ratio.detach().clamp(1 - clip_low, 1 + clip_high)
+    moved = lp - torch.where(live, old_logps, 0).double()
+    ratio = moved.detach().exp()
+    held = ratio.clamp(1 - clip_low, 1 + clip_high)
     moves = torch.where(A > 0, ~(ratio > 1 + clip_high), ~(ratio < 1 - clip_low))
+    # what the clip holds has no gradient, be the ratio +inf
+    ratio = torch.where(moves, moved, 0.0).exp()
     rows = -torch.where(moves, ratio * A, held * A)
     kl = torch.zeros_like(lp)
     if ref_logps is not None:
