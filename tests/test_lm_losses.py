@@ -806,6 +806,22 @@ def test_policy_impossible_old_tokens(device):
 
 
 @pytest.mark.parametrize("device", CPU_GPU)
+def test_policy_nan_advantage_is_nan(device):
+    """A NaN advantage makes its token's loss a NaN, and its gradient with it,
+    on whichever side of the clip the ratio lies."""
+    need(device)
+    x = make_logits(1, 4, 33, torch.float32, device)
+    actions, old, adv, _ = make_rollout(x, spread=0.0)
+    old = old - torch.tensor([0.0, 2.0, -2.0, 0.0], device=device)
+    adv[0, :3] = float("nan")
+    x.requires_grad_(True)
+    out = policy_loss(x, actions, old, adv, reduction="none")
+    g, = torch.autograd.grad(out.loss.sum(), x)
+    assert torch.isnan(out.loss[0, :3]).all() and torch.isfinite(out.loss[0, 3])
+    assert torch.isnan(g[0, :3]).all() and torch.isfinite(g[0, 3]).all()
+
+
+@pytest.mark.parametrize("device", CPU_GPU)
 def test_policy_kl_without_weight(device):
     """With a coefficient of 0 the KL is reported only, and one that passes the
     largest number changes neither loss nor gradient."""

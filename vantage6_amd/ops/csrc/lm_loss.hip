@@ -610,7 +610,7 @@ __global__ void __launch_bounds__(kThreads)
     const double ratio = exp(lp - (double)po.old_lp[r]);
     const double held = fmin(fmax(ratio, lo), hi);
     // the lesser of ratio*A and held*A; a NaN stays one
-    const bool moves = A > 0.0 ? !(ratio > hi) : !(ratio < lo);
+    const bool moves = A > 0.0 ? !(ratio > hi) : !(ratio < lo) || A != A;
     loss = moves ? -ratio * A : -held * A;
     by_lp = moves ? -ratio * A : 0.0;
     if (po.ref_lp) {

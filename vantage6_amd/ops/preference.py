@@ -146,6 +146,7 @@ def policy_loss(logits: torch.Tensor, actions: torch.Tensor,
     ratio = moved.detach().exp()
     held = ratio.clamp(1 - clip_low, 1 + clip_high)
     moves = torch.where(A > 0, ~(ratio > 1 + clip_high), ~(ratio < 1 - clip_low))
+    moves = moves | A.isnan()  # a NaN stays one
     # what the clip holds has no gradient, be the ratio +inf
     ratio = torch.where(moves, moved, 0.0).exp()
     rows = -torch.where(moves, ratio * A, held * A)
