@@ -439,6 +439,38 @@ def test_distill_extreme_logits_at_low_temperatures(device, dtype, t):
 
 
 @pytest.mark.parametrize("device", CPU_GPU)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("t", [0.3, 1.0])
+def test_distill_places_far_apart(device, dtype, t):
+    """A masked logit in the record costs its own probability's worth, not
+    infinity; below a logit of the largest value the others keep their shares."""
+    need(device)
+    V = 300
+    fi = torch.finfo(dtype)
+    x = make_logits(1, 2, V, dtype, "cpu")
+    values, indices, _ = make_record(x, 9, t, tail=False)
+    lse = torch.logsumexp(values.double() / t, -1).float() + 0.4
+    x[0, 0, indices[0, 0, 3]] = fi.min
+    values[0, 0, 3] = -200.0 * t
+    args = [a.to(device) for a in (x, values, indices)]
+    check_distill(*[a[:, :1] for a in args], None, t)
+    check_distill(*[a[:, :1] for a in args], lse[:, :1].to(device), t)
+    x[0, 1, indices[0, 1, 0]] = fi.max  # all the student's mass is on one place
+    y = x[:, 1:].to(device).requires_grad_(True)
+    loss = distill_loss(y, values[:, 1:].to(device), indices[:, 1:].to(device),
+                        lse[:, 1:].to(device), temperature=t)
+    got, = torch.autograd.grad(loss, y, torch.tensor(64.0, device=device))
+    p = (values[0, 1].double() / t - lse[0, 1].double()).exp()
+    rest, out = 1 - p.sum(), x[0, 1].double().index_fill(0, indices[0, 1], -math.inf)
+    want = -rest * torch.softmax(out / t, -1)
+    want[indices[0, 1]] = -p
+    want[indices[0, 1, 0]] += 1.0
+    assert torch.isfinite(loss)
+    # sums of a place's p and the rest's share: as any gradient, q being the shares
+    check_grad(got[0], want[None] * 64.0 * t, torch.tensor([64.0 * t]), want.abs()[None])
+
+
+@pytest.mark.parametrize("device", CPU_GPU)
 @pytest.mark.parametrize("tail", [False, True])
 def test_distill_unlikely_index_outside_is_nan(device, tail):
     """An index outside the row is one however small its probability; a value

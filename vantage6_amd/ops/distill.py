@@ -123,12 +123,13 @@ def _distill_reference(logits, values, indices, lse, t, mask, reduction):
     on = live[..., None]
     x = torch.where(on, logits, 0).to(reference_dtype(logits))
     top = x.detach().amax(-1, keepdim=True).clamp_min(torch.finfo(x.dtype).min)
-    x = (x - top) / t  # in this order: the type's lowest value stays a number
     at = indices.clamp(0, V - 1)
     inside = torch.zeros(logits.shape, dtype=torch.int32, device=logits.device)
     inside = inside.scatter_add(-1, at, (present & (indices < V)).int()) > 0
-    log_s = torch.logsumexp(x, -1, keepdim=True)
-    log_q = x.gather(-1, at) - log_s
+    # subtracted before the division, and single places in 64 bits: the type's
+    # lowest value stays a number
+    log_s = torch.logsumexp((x - top) / t, -1, keepdim=True).double()
+    log_q = (x.gather(-1, at).double() - top.double()) / t - log_s
     v = v.masked_fill(~some, float("-inf")).masked_fill(~on, 0.0)
     log_p = v - (torch.logsumexp(v, -1, keepdim=True) if lse is None
                  else lse.double()[..., None])
@@ -140,7 +141,11 @@ def _distill_reference(logits, values, indices, lse, t, mask, reduction):
         rest = (1.0 - p.sum(-1)).clamp_min(0.0)
         out = x.masked_fill(inside, float("-inf"))
         any_out = (out > float("-inf")).any(-1) | out.isnan().any(-1)
-        log_out = torch.logsumexp(torch.where(any_out[..., None], out, 0.0), -1)
+        out = torch.where(any_out[..., None], out, 0.0)
+        # by a maximum of its own: far below the record its shares still differ
+        low = out.detach().amax(-1, keepdim=True).clamp_min(torch.finfo(x.dtype).min)
+        log_out = torch.logsumexp((out - low) / t, -1).double() + (
+            (low.double() - top.double()) / t)[..., 0]
         rows = rows + torch.where(any_out, torch.xlogy(rest, rest)
                                   - rest * (log_out - log_s[..., 0]), 0.0)
     rows = rows * torch.where((some & (indices >= V)).any(-1), float("nan"), 1.0)
