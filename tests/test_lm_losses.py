@@ -1455,6 +1455,42 @@ def test_record_of_another_temperature(device):
                     run()
 
 
+@pytest.mark.parametrize("device", CPU_GPU)
+def test_record_goes_into_the_loss_as_it_is(device):
+    """``distill_loss(logits, **teacher_record(...))``: the record's entries are
+    the loss's arguments, its temperature among them."""
+    need(device)
+    from vantage6_amd.models import build_model, teacher_record
+
+    torch.manual_seed(1)
+    kw = TINY["llama_1b"]
+    model = build_model("llama_1b", device=device, **kw)
+    ids = torch.randint(0, kw["vocab"], (2, 8), generator=torch.Generator().manual_seed(2))
+    record = teacher_record(model, ids.to(device), 5, 2.0)
+    x = make_logits(2, 8, kw["vocab"], torch.float32, device)
+    want = distill_loss(x, record["teacher_values"], record["teacher_indices"],
+                        record["teacher_lse"], temperature=2.0)
+    assert torch.isfinite(want) and torch.equal(distill_loss(x, **record, temperature=2.0), want)
+    assert torch.isnan(distill_loss(x, **record))  # at 1
+    record["teacher_temperature"][0] = 1.0
+    each = distill_loss(x, **record, reduction="none")
+    assert torch.isfinite(each[0]).all() and torch.isnan(each[1]).all()
+    mask = torch.tensor([[True], [False]], device=device).expand(2, 8)
+    assert torch.isfinite(distill_loss(x, **record, mask=mask))
+    lone = {k: v[0, 3] for k, v in record.items() if v.dim() > 1}
+    one = torch.ones((), dtype=torch.float64, device=device)
+    for shape, made in (((131,), one), ((1, 1, 1, 131), one.view(1))):
+        args = {k: v.reshape((*shape[:-1], *v.shape)) for k, v in lone.items()}
+        y = x[0, 3].reshape(shape)
+        assert torch.isfinite(distill_loss(y, **args, teacher_temperature=made))
+        assert torch.isnan(distill_loss(y, **args, teacher_temperature=made, temperature=0.7))
+    no_lse = {k: v for k, v in record.items() if k != "teacher_lse"}
+    assert torch.isfinite(distill_loss(x, **no_lse, temperature=0.7))
+    for bad in (torch.ones(8, device=device), torch.ones(2, dtype=torch.int64, device=device)):
+        with pytest.raises(ValueError):
+            distill_loss(x, **{**record, "teacher_temperature": bad})
+
+
 def test_objective_refusals():
     from algorithms.fedavg import fit_rounds
     from vantage6_amd.models import model_loss

@@ -51,19 +51,14 @@ def _lm_logits(model, ids):
 def _distill_objective(options) -> Callable:
     """Batch: ``input_ids`` [N, S] and the teacher's record of every position,
     ``teacher_values`` and ``teacher_indices`` [N, S, k], optionally
-    ``teacher_lse`` and ``mask`` [N, S]. With ``teacher_temperature`` [N] a
-    ``teacher_lse`` of another temperature than the loss's makes the loss NaN,
-    as a device cannot raise."""
+    ``teacher_lse`` and ``mask`` [N, S], and ``teacher_temperature`` [N]."""
     def loss(model, batch):
         from ..ops.distill import distill_loss
 
-        lse = batch.get("teacher_lse")
-        if lse is not None and "teacher_temperature" in batch:
-            same = batch["teacher_temperature"] == options.get("temperature", 1.0)
-            lse = torch.where(same[:, None], lse, float("nan"))
         return distill_loss(
             _lm_logits(model, batch["input_ids"]), batch["teacher_values"],
-            batch["teacher_indices"], lse, mask=batch.get("mask"), **options)
+            batch["teacher_indices"], batch.get("teacher_lse"), mask=batch.get("mask"),
+            teacher_temperature=batch.get("teacher_temperature"), **options)
 
     return loss
 

@@ -70,7 +70,8 @@ def distill_loss(logits: torch.Tensor, teacher_values: torch.Tensor,
                  teacher_indices: torch.Tensor,
                  teacher_lse: torch.Tensor | None = None, *,
                  temperature: float = 1.0, mask: torch.Tensor | None = None,
-                 reduction: str = "mean") -> torch.Tensor:
+                 reduction: str = "mean",
+                 teacher_temperature: torch.Tensor | None = None) -> torch.Tensor:
     """Divergence of ``logits`` ``[..., V]`` from a teacher's records, fp32.
 
     ``teacher_values`` and ``teacher_indices`` are ``[..., k]`` with k <= 256,
@@ -81,6 +82,10 @@ def distill_loss(logits: torch.Tensor, teacher_values: torch.Tensor,
     its logits hold) where ``mask`` is False, and then its logits are not read,
     or where its record holds nothing. An index of V or more makes the row's
     loss and gradient NaN.
+
+    ``teacher_lse`` holds at one temperature. ``teacher_temperature``, of the
+    rows' first dimension, says which: where it is not ``temperature`` the rows'
+    losses are NaN, as a device cannot raise.
 
     ``reduction``: "mean" over the rows that count, "sum", or "none" (a loss
     per row). The record is a constant of the loss."""
@@ -95,6 +100,12 @@ def distill_loss(logits: torch.Tensor, teacher_values: torch.Tensor,
     check_rows("teacher_values", teacher_values, logits, (*rows, k), True)
     if teacher_lse is not None:
         check_rows("teacher_lse", teacher_lse, logits, rows, True)
+    if teacher_temperature is not None:
+        check_rows("teacher_temperature", teacher_temperature, logits, rows[:1], True)
+        if teacher_lse is not None:
+            same = teacher_temperature == temperature
+            same = same.reshape(rows[:1] + (1,) * (len(rows) - 1))
+            teacher_lse = torch.where(same, teacher_lse, float("nan"))
     if mask is not None:
         check_mask(mask, logits, rows)
     if logits.is_cuda:
